@@ -131,7 +131,8 @@ def _keys(rows, kv_heads, dim, gen):
 def _quantised(x):
     """(codes, scales): one scale per row of the last dimension."""
     x = x.float()
-    scale = x.abs().amax(-1).clamp(min=1e-8) / FP8_MAX
+    amax = x.abs().amax(-1).clamp(min=1e-8)
+    scale = amax / torch.full_like(amax, FP8_MAX)         # (by a tensor: a true division, where one by a number multiplies by 1 / 448)
     return (x / scale[..., None]).clamp(-FP8_MAX, FP8_MAX).to(FP8), scale
 
 
