@@ -295,6 +295,67 @@ int fp8lin_mlp_w8a8_preq(const void* xq, const void* w_gate_up, const float* gat
                          const float* down_scale, const float* down_input_scale, const void* down_bias, void* y, int64_t ldy,
                          int64_t M, int64_t H, int64_t I, int64_t N, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- paged key-value cache and the attention of a decode step ------------------------------------------
+ * The cache that the reference's engine keeps per layer and its attention kernels read (nanovllm/layers/attention.py:25-62
+ * store_kvcache, :206 and :312 the paged decode attention; nanovllm/layers/kv_cache_kernels.py:21-134 the quantised store and
+ * its way back), for one pair of storage types:
+ *   FP8LIN_CACHE_BF16   keys and values as they are;
+ *   FP8LIN_CACHE_E4M3   e4m3 codes with one fp32 scale per token and head, made as the row is written:
+ *                       scale = max(max_d |x_d|, 1e-8) / 448;  code = RNE(clamp(x / scale, +-448)), a true division.
+ * k, v: [num_blocks][block_size][num_kv_heads][head_dim], head_dim contiguous, the other strides (in elements, shared by k and
+ * v) free but multiples of 16 bytes; k_scale, v_scale: fp32 [num_blocks][block_size][num_kv_heads] with free strides (shared),
+ * NULL for bf16.  k and v 16-byte aligned; head_dim a multiple of 16 from 16 to 256.  Any block_size of at least 1; pages that hold
+ * a multiple of 16 tokens are read faster, and fastest with the tokens of a head one behind the other ([block][head][token][dim] in memory).
+ * Token i of a sequence lies at offset i % block_size of page block_tables[i / block_size]; slot = page * block_size + offset.
+ * A slot or page outside the cache is not touched: the call reports it in its workspace's status word (0x201; fp8lin_read_status,
+ * and in Python the next call on the stream raises). */
+enum { FP8LIN_CACHE_BF16 = 0, FP8LIN_CACHE_E4M3 = 1 };
+typedef struct fp8lin_kv_cache {
+    void* k;
+    void* v;
+    float* k_scale;
+    float* v_scale;
+    int64_t num_blocks;
+    int64_t stride_block, stride_token, stride_head;                      /* of k and v */
+    int64_t scale_stride_block, scale_stride_token, scale_stride_head;    /* of k_scale and v_scale */
+    int block_size, num_kv_heads, head_dim;
+    int dtype;                                                            /* FP8LIN_CACHE_* */
+} fp8lin_kv_cache;
+
+/* Row t of k and v (bf16 [tokens][num_kv_heads][head_dim], strides of tokens and heads in elements, multiples of 8; 16-byte
+ * aligned) goes to slot slot_mapping[t]; a negative slot is skipped.  The slots of one call have to be distinct: where two
+ * rows name one slot, what it holds afterwards may be mixed from both.  workspace: at least FP8LIN_WS_HEADER_BYTES. */
+int fp8lin_kv_cache_write(const fp8lin_kv_cache* cache, const void* k, int64_t k_stride_token, int64_t k_stride_head,
+                          const void* v, int64_t v_stride_token, int64_t v_stride_head, const int32_t* slot_mapping,
+                          int64_t tokens, void* workspace, size_t workspace_bytes, void* stream);
+
+/* The first tokens of `batch` sequences as bf16 rows, one sequence behind the other: row r of k and v (bf16
+ * [rows][num_kv_heads][head_dim], strides as above) is token r - cu_seqlens[b] of the sequence b with
+ * cu_seqlens[b] <= r < cu_seqlens[b + 1]; e4m3: bf16(code * scale).  cu_seqlens: int32 [batch + 1] on the device, from 0 on, not falling.
+ * Rows from cu_seqlens[batch] on are left as they were.  block_tables: int32 [batch][ld_tables], of which max_pages entries
+ * per sequence may be read (entries behind a sequence's last page may hold anything).  workspace: at least the header. */
+int fp8lin_kv_cache_read(const fp8lin_kv_cache* cache, const int32_t* block_tables, int64_t ld_tables, int64_t max_pages,
+                         const int32_t* cu_seqlens, int64_t batch, void* k, int64_t k_stride_token, int64_t k_stride_head,
+                         void* v, int64_t v_stride_token, int64_t v_stride_head, int64_t rows, void* workspace,
+                         size_t workspace_bytes, void* stream);
+
+/* Attention of one new token per sequence (which is in the cache already) over its first context_lens[b] tokens:
+ *   out[b][h] = sum_i softmax_i(scale * q[b][h] . K[i][h / group]) V[i][h / group],   group = num_heads / num_kv_heads,
+ * a context of 0 (or less) gives zeros.  Products of bf16 (or e4m3) values are exact and sums, statistics and scales fp32.
+ * q: bf16 [batch][num_heads][head_dim], strides in elements, multiples of 8, 16-byte aligned.  out_scale NULL: out is bf16
+ * [batch][num_heads * head_dim] with rows ld_out elements apart (a multiple of 8; 16-byte aligned); else out is u8, the e4m3
+ * codes that fp8lin_quantize_activation makes of the bf16 result with *out_scale (one float on the device).
+ * A context is read through max_pages entries of its table at most: longer ones are cut there and reported like a bad page.
+ * Results do not depend on what other sequences of the batch hold in their pages, nor on the order in which blocks run, but
+ * the split of a long sequence (and with it the last bits) depends on the lengths of the whole batch.  An infinity or NaN among a sequence's own keys and values makes what
+ * it reaches non-finite; nothing behind a context's end is read.
+ * workspace: fp8lin_paged_attention_workspace_bytes, zero-filled once, rules as for the linears. */
+size_t fp8lin_paged_attention_workspace_bytes(int64_t num_heads, int64_t num_kv_heads, int64_t head_dim, int dtype);
+int fp8lin_paged_attention(const fp8lin_kv_cache* cache, const void* q, int64_t q_stride_row, int64_t q_stride_head,
+                           const int32_t* block_tables, int64_t ld_tables, int64_t max_pages, const int32_t* context_lens,
+                           int64_t batch, int64_t num_heads, float scale, const float* out_scale, void* out, int64_t ld_out,
+                           void* workspace, size_t workspace_bytes, void* stream);
+
 /* The route of a shape by its tile counts alone ("stream_mma_w8a8_m16", "umma_w8a8_128x256", ...): what calls run that the
  * CTA-pair kernels with channels as the MMA's M do not take -- several destinations, N or ldy not a multiple of 8, y not
  * 16-byte aligned.  Not what most other calls of 17 rows and more run: see fp8lin_kernel_name.  Host-only, static string. */
@@ -328,7 +389,7 @@ int fp8lin_set_tuning(const char* knob, int value);
  * `stream`) and clears it.  0 = no kernel gave up a bounded wait.  Otherwise the code of the wait
  * that ran out (about a second): 0x101 operand tile never landed, 0x102 ring slot never freed, 0x103 /
  * 0x104 accumulator never filled / never drained, 0x105 in-kernel activation quantiser, 0x106 a peer
- * CTA of the cluster (split-K hand-over) never answered.
+ * CTA of the cluster (split-K hand-over) never answered.  0x201: a cache call met a slot or a page outside the cache.
  *
  * The call whose kernel gave up has no valid result.  To learn of it without a blocking read, put the address of an int
  * that the device can write and the host can read (pinned, mapped memory; initially 0) into bytes 8..15 of the workspace,

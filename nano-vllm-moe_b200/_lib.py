@@ -17,6 +17,8 @@ HOST_PATH = LIB_PATH.parent / "_fp8host.so"
 
 W8A16 = 0
 W8A8_STATIC = 1
+CACHE_BF16 = 0
+CACHE_E4M3 = 1
 WS_HEADER_BYTES = 65536
 
 OK, ERR_NULL, ERR_SHAPE, ERR_ALIGN, ERR_WORKSPACE, ERR_ARCH, ERR_LAUNCH, ERR_DEVICE, ERR_ARG = range(9)
@@ -70,11 +72,29 @@ SIGNATURES = {
                                         c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int64, c_int64, c_void_p,
                                         c_int64, c_void_p, c_size_t, c_void_p]),
     "fp8lin_moe_combine": (c_int, [c_void_p, c_void_p, c_int64, c_int, c_int64, c_void_p]),
+    "fp8lin_kv_cache_write": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_int64,
+                                      c_void_p, c_size_t, c_void_p]),
+    "fp8lin_kv_cache_read": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int64,
+                                     c_void_p, c_int64, c_int64, c_int64, c_void_p, c_size_t, c_void_p]),
+    "fp8lin_paged_attention_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int64, c_int]),
+    "fp8lin_paged_attention": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64,
+                                       ctypes.c_float, c_void_p, c_void_p, c_int64, c_void_p, c_size_t, c_void_p]),
     "fp8lin_variant_name": (c_char_p, [c_int, c_int64, c_int64, c_int64]),
     "fp8lin_kernel_name": (c_char_p, [c_int, c_int64, c_int64, c_int64]),
     "fp8lin_set_tuning": (c_int, [c_char_p, c_int]),
     "fp8lin_read_status": (c_int, [c_void_p, c_void_p, POINTER(c_int)]),
 }
+
+
+
+class KvCache(ctypes.Structure):
+    """``fp8lin_kv_cache`` of include/fp8lin.h."""
+
+    _fields_ = [("k", c_void_p), ("v", c_void_p), ("k_scale", c_void_p), ("v_scale", c_void_p), ("num_blocks", c_int64),
+                ("stride_block", c_int64), ("stride_token", c_int64), ("stride_head", c_int64),
+                ("scale_stride_block", c_int64), ("scale_stride_token", c_int64), ("scale_stride_head", c_int64),
+                ("block_size", c_int), ("num_kv_heads", c_int), ("head_dim", c_int), ("dtype", c_int)]
+
 
 _lib = None
 

@@ -1291,6 +1291,7 @@ int fp8lin_read_status(void* workspace, void* stream, int* status_out) {
     if (v != 0) {
         cudaMemsetAsync(workspace, 0, sizeof(int), st);
         cudaStreamSynchronize(st);
+        if (v == kDevBadPage) return fail(FP8LIN_ERR_DEVICE, "a kernel met a slot or page outside the key-value cache (device status 0x%x)", v);
         return fail(FP8LIN_ERR_DEVICE, "a kernel gave up a bounded wait (device status 0x%x)", v);
     }
     return FP8LIN_OK;

@@ -35,7 +35,8 @@ __host__ __device__ inline WsView ws_view(void* ws, size_t bytes) {
 
 // device status codes written by kernels that gave up a bounded wait
 enum : int { kDevOk = 0, kDevTimeoutFull = 0x101, kDevTimeoutEmpty = 0x102, kDevTimeoutTmemFull = 0x103,
-             kDevTimeoutTmemEmpty = 0x104, kDevTimeoutQuant = 0x105, kDevTimeoutPeer = 0x106 };
+             kDevTimeoutTmemEmpty = 0x104, kDevTimeoutQuant = 0x105, kDevTimeoutPeer = 0x106,
+             kDevBadPage = 0x201 };     // (not a wait: a slot or page outside the key-value cache)
 
 // A wait that gave up leaves its code in the status word, and in the host's word whose address the header holds (the words
 // behind the status: kWsHostWord; 0 = none), which a caller can look at on every call without asking the device.

@@ -18,6 +18,7 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <cmath>
 #include <cstdio>
 #include <map>
 #include <mutex>
@@ -62,6 +63,7 @@ struct Scratch {
     std::map<std::pair<int, void*>, StreamScratch> live;
     std::vector<at::Tensor> retired;
 };
+constexpr int kBadPage = 0x201;              // the status of a cache call, not of a wait
 constexpr int64_t kHostWordAt = 8;           // byte of the header that names the host's word
 Scratch& scratch() { static Scratch* s = new Scratch; return *s; }      // (outlives the CUDA context's teardown)
 
@@ -75,6 +77,9 @@ Scratch& scratch() { static Scratch* s = new Scratch; return *s; }      // (outl
     }
     char hex[16];
     snprintf(hex, sizeof(hex), "0x%x", code);
+    if (code == kBadPage)
+        throw std::runtime_error("an earlier call on this stream met a slot or page outside the key-value cache: it was not touched, and what "
+                                 "the call returned for it is not valid");
     throw std::runtime_error(std::string("a kernel of an earlier call on this stream gave up a bounded wait (device status ") + hex +
                              "): the result of that call is not valid");
 }
@@ -470,6 +475,182 @@ PyObject* py_moe_block(PyObject*, PyObject* const* a, Py_ssize_t na) {
     });
 }
 
+// ---- paged key-value cache ---------------------------------------------------------------------------------------------
+
+void need_device(const at::Tensor& t, const c10::Device& device, const char* what) {
+    need_cuda(t);
+    if (t.device() != device) throw ValueError(std::string(what) + " is on another device than the cache");
+}
+
+// The same steps through memory, wherever there is more than one element to step over.
+bool same_strides(const at::Tensor& a, const at::Tensor& b) {
+    for (int64_t d = 0; d < a.dim(); ++d)
+        if (a.size(d) > 1 && a.stride(d) != b.stride(d)) return false;
+    return true;
+}
+
+fp8lin_kv_cache cache_of(const at::Tensor& k, const at::Tensor& v, const at::Tensor* ks, const at::Tensor* vs) {
+    need_cuda(k);
+    need_device(v, k.device(), "v_cache");
+    const bool e4m3 = k.scalar_type() == at::kFloat8_e4m3fn || k.scalar_type() == at::kByte;
+    if ((!e4m3 && k.scalar_type() != at::kBFloat16) || v.scalar_type() != k.scalar_type())
+        throw ValueError("k_cache and v_cache must both be bfloat16, or both e4m3 codes (float8_e4m3fn or uint8)");
+    if (k.dim() != 4 || v.sizes() != k.sizes() || k.stride(3) != 1 || v.stride(3) != 1 || !same_strides(k, v))
+        throw ValueError("k_cache and v_cache must be [num_blocks, block_size, num_kv_heads, head_dim] with the same strides and contiguous rows");
+    if (e4m3 != (ks != nullptr) || e4m3 != (vs != nullptr))
+        throw ValueError(e4m3 ? "an e4m3 cache needs k_scale and v_scale" : "a bfloat16 cache has no scales");
+    if (k.size(1) > INT32_MAX || k.size(2) > INT32_MAX || k.size(3) > INT32_MAX) throw ValueError("the cache is too large");
+    fp8lin_kv_cache c = {};
+    c.k = k.mutable_data_ptr();
+    c.v = v.mutable_data_ptr();
+    c.num_blocks = k.size(0);
+    c.block_size = (int)k.size(1);
+    c.num_kv_heads = (int)k.size(2);
+    c.head_dim = (int)k.size(3);
+    c.stride_block = k.stride(0);
+    c.stride_token = k.stride(1);
+    c.stride_head = k.stride(2);
+    c.dtype = e4m3 ? FP8LIN_CACHE_E4M3 : FP8LIN_CACHE_BF16;
+    if (e4m3) {
+        need_device(*ks, k.device(), "k_scale");
+        need_device(*vs, k.device(), "v_scale");
+        if (ks->scalar_type() != at::kFloat || vs->scalar_type() != at::kFloat || ks->dim() != 3 || ks->sizes() != k.sizes().slice(0, 3) ||
+            vs->sizes() != ks->sizes() || !same_strides(*ks, *vs))
+            throw ValueError("k_scale and v_scale must be float32 [num_blocks, block_size, num_kv_heads] with the same strides");
+        c.k_scale = ks->mutable_data_ptr<float>();
+        c.v_scale = vs->mutable_data_ptr<float>();
+        c.scale_stride_block = ks->stride(0);
+        c.scale_stride_token = ks->stride(1);
+        c.scale_stride_head = ks->stride(2);
+    }
+    return c;
+}
+
+const int32_t* int32_of(const at::Tensor& t, int64_t dims, const c10::Device& device, const char* what) {
+    need_device(t, device, what);
+    if (t.scalar_type() != at::kInt || t.dim() != dims || (t.size(dims - 1) > 1 && t.stride(dims - 1) != 1))
+        throw ValueError(std::string(what) + " must be an int32 tensor of " + std::to_string(dims) + (dims == 1 ? " dimension" : " dimensions") + " with contiguous rows");
+    return (const int32_t*)t.const_data_ptr();
+}
+
+void check_heads(const at::Tensor& x, int64_t heads, int64_t dim, const c10::Device& device, const char* what) {
+    need_device(x, device, what);
+    if (x.scalar_type() != at::kBFloat16 || x.dim() != 3 || x.size(1) != heads || x.size(2) != dim || x.stride(2) != 1)
+        throw ValueError(std::string(what) + " must be bfloat16 [rows, " + std::to_string(heads) + ", " + std::to_string(dim) + "] with contiguous channels");
+}
+
+// kv_cache_write(k, v, slot_mapping, k_cache, v_cache, k_scale | None, v_scale | None)
+PyObject* py_kv_cache_write(PyObject*, PyObject* const* a, Py_ssize_t na) {
+    return guarded([&]() -> PyObject* {
+        need_args(na, 7, "kv_cache_write");
+        const at::Tensor& k = tensor(a[0], "k");
+        const at::Tensor& v = tensor(a[1], "v");
+        const at::Tensor& slots = tensor(a[2], "slot_mapping");
+        const at::Tensor& kc = tensor(a[3], "k_cache");
+        const fp8lin_kv_cache c = cache_of(kc, tensor(a[4], "v_cache"), optional_tensor(a[5], "k_scale"), optional_tensor(a[6], "v_scale"));
+        const c10::Device on = kc.device();
+        check_heads(k, c.num_kv_heads, c.head_dim, on, "k");
+        check_heads(v, c.num_kv_heads, c.head_dim, on, "v");
+        const int32_t* sp = int32_of(slots, 1, on, "slot_mapping");
+        if (v.size(0) != k.size(0) || slots.size(0) != k.size(0)) throw ValueError("k, v and slot_mapping must have the same number of rows");
+        const c10::cuda::CUDAGuard device(on);
+        const auto stream = c10::cuda::getCurrentCUDAStream();
+        const at::Tensor scr = workspace(stream, FP8LIN_WS_HEADER_BYTES);
+        const int rc = unlocked([&] {
+            return fp8lin_kv_cache_write(&c, k.const_data_ptr(), k.stride(0), k.stride(1), v.const_data_ptr(), v.stride(0), v.stride(1), sp, k.size(0),
+                                         scr.mutable_data_ptr(), (size_t)scr.numel(), stream.stream());
+        });
+        check(rc, "fp8lin_kv_cache_write");
+        Py_RETURN_NONE;
+    });
+}
+
+// kv_cache_read(k_cache, v_cache, block_tables, cu_seqlens, rows, k_scale | None, v_scale | None, k_out | None, v_out | None) -> (k, v)
+PyObject* py_kv_cache_read(PyObject*, PyObject* const* a, Py_ssize_t na) {
+    return guarded([&]() -> PyObject* {
+        need_args(na, 9, "kv_cache_read");
+        const at::Tensor& kc = tensor(a[0], "k_cache");
+        const fp8lin_kv_cache c = cache_of(kc, tensor(a[1], "v_cache"), optional_tensor(a[5], "k_scale"), optional_tensor(a[6], "v_scale"));
+        const c10::Device on = kc.device();
+        const at::Tensor& tables = tensor(a[2], "block_tables");
+        const at::Tensor& cu = tensor(a[3], "cu_seqlens");
+        const int32_t* tp = int32_of(tables, 2, on, "block_tables");
+        const int32_t* cp = int32_of(cu, 1, on, "cu_seqlens");
+        const int64_t rows = PyLong_AsLongLong(a[4]);
+        if (PyErr_Occurred()) return nullptr;
+        if (rows < 0) throw ValueError("rows must not be negative");
+        if (cu.size(0) != tables.size(0) + 1) throw ValueError("cu_seqlens must have one value more than block_tables has rows");
+        const at::Tensor* ko = optional_tensor(a[7], "k_out");
+        const at::Tensor* vo = optional_tensor(a[8], "v_out");
+        const c10::cuda::CUDAGuard device(on);
+        const at::Tensor k = ko ? *ko : empty({rows, c.num_kv_heads, c.head_dim}, at::kBFloat16, on);
+        const at::Tensor v = vo ? *vo : empty({rows, c.num_kv_heads, c.head_dim}, at::kBFloat16, on);
+        check_heads(k, c.num_kv_heads, c.head_dim, on, "k_out");
+        check_heads(v, c.num_kv_heads, c.head_dim, on, "v_out");
+        if (k.size(0) != rows || v.size(0) != rows) throw ValueError("k_out and v_out must have the given number of rows");
+        const auto stream = c10::cuda::getCurrentCUDAStream();
+        const at::Tensor scr = workspace(stream, FP8LIN_WS_HEADER_BYTES);
+        const int rc = unlocked([&] {
+            return fp8lin_kv_cache_read(&c, tp, tables.stride(0), tables.size(1), cp, tables.size(0), k.mutable_data_ptr(), k.stride(0), k.stride(1),
+                                        v.mutable_data_ptr(), v.stride(0), v.stride(1), rows, scr.mutable_data_ptr(), (size_t)scr.numel(), stream.stream());
+        });
+        check(rc, "fp8lin_kv_cache_read");
+        PyObject* t = PyTuple_New(2);
+        if (!t) return nullptr;
+        PyTuple_SET_ITEM(t, 0, THPVariable_Wrap(k));
+        PyTuple_SET_ITEM(t, 1, THPVariable_Wrap(v));
+        return t;
+    });
+}
+
+// paged_attention(q, k_cache, v_cache, block_tables, context_lens, scale, k_scale | None, v_scale | None, out_scale | None, out | None)
+//     -> out [B, H, D], bf16 or codes
+PyObject* py_paged_attention(PyObject*, PyObject* const* a, Py_ssize_t na) {
+    return guarded([&]() -> PyObject* {
+        need_args(na, 10, "paged_attention");
+        const at::Tensor& q = tensor(a[0], "q");
+        const at::Tensor& kc = tensor(a[1], "k_cache");
+        const fp8lin_kv_cache c = cache_of(kc, tensor(a[2], "v_cache"), optional_tensor(a[6], "k_scale"), optional_tensor(a[7], "v_scale"));
+        const c10::Device on = kc.device();
+        const at::Tensor& tables = tensor(a[3], "block_tables");
+        const at::Tensor& lens = tensor(a[4], "context_lens");
+        const int32_t* tp = int32_of(tables, 2, on, "block_tables");
+        const int32_t* lp = int32_of(lens, 1, on, "context_lens");
+        if (q.dim() != 3) throw ValueError("q must be bfloat16 [batch, num_heads, head_dim]");
+        const int64_t batch = q.size(0), heads = q.size(1);
+        check_heads(q, heads, c.head_dim, on, "q");
+        if (tables.size(0) != batch || lens.size(0) != batch) throw ValueError("q, block_tables and context_lens must have the same number of rows");
+        const double scale = a[5] == Py_None ? 1.0 / std::sqrt((double)c.head_dim) : PyFloat_AsDouble(a[5]);
+        if (PyErr_Occurred()) return nullptr;
+        const at::Tensor* os = optional_tensor(a[8], "out_scale");
+        const at::Tensor* out = optional_tensor(a[9], "out");
+        if (os) {
+            check_scale(*os, "out_scale");
+            need_device(*os, on, "out_scale");
+        }
+        const at::ScalarType dtype = os ? at::kByte : at::kBFloat16;
+        const c10::cuda::CUDAGuard device(on);
+        const at::Tensor y = out ? *out : empty({batch, heads, c.head_dim}, dtype, on);
+        const int64_t row = heads * c.head_dim;
+        if (out) {
+            need_device(y, on, "out");
+            const bool matrix = y.dim() == 2 && y.size(0) == batch && y.size(1) == row && y.stride(1) == 1;
+            const bool by_head = y.dim() == 3 && y.size(0) == batch && y.size(1) == heads && y.size(2) == c.head_dim && y.stride(2) == 1 &&
+                                 (heads == 1 || y.stride(1) == c.head_dim);
+            if (y.scalar_type() != dtype || (!matrix && !by_head))
+                throw ValueError(std::string("out must be ") + (os ? "uint8" : "bfloat16") + " [batch, num_heads, head_dim] or [batch, num_heads * head_dim] with contiguous rows");
+        }
+        const auto stream = c10::cuda::getCurrentCUDAStream();
+        const at::Tensor scr = workspace(stream, fp8lin_paged_attention_workspace_bytes(heads, c.num_kv_heads, c.head_dim, c.dtype));
+        const int rc = unlocked([&] {
+            return fp8lin_paged_attention(&c, q.const_data_ptr(), q.stride(0), q.stride(1), tp, tables.stride(0), tables.size(1), lp, batch, heads, (float)scale,
+                                          (const float*)ptr(os), y.mutable_data_ptr(), y.stride(0), scr.mutable_data_ptr(), (size_t)scr.numel(), stream.stream());
+        });
+        check(rc, "fp8lin_paged_attention");
+        return THPVariable_Wrap(y);
+    });
+}
+
 // workspace(device_index, stream_handle, nbytes, for_status) -> the stream's scratch tensor.  for_status: to read the status
 // word, so a wait that was given up is not raised here, and the host's copy of its code is forgotten.
 PyObject* py_workspace(PyObject*, PyObject* const* a, Py_ssize_t na) {
@@ -509,6 +690,9 @@ PyMethodDef kMethods[] = {
     {"mlp", (PyCFunction)(void (*)(void))py_mlp, METH_FASTCALL, nullptr},
     {"moe_route", (PyCFunction)(void (*)(void))py_moe_route, METH_FASTCALL, nullptr},
     {"moe_block", (PyCFunction)(void (*)(void))py_moe_block, METH_FASTCALL, nullptr},
+    {"kv_cache_write", (PyCFunction)(void (*)(void))py_kv_cache_write, METH_FASTCALL, nullptr},
+    {"kv_cache_read", (PyCFunction)(void (*)(void))py_kv_cache_read, METH_FASTCALL, nullptr},
+    {"paged_attention", (PyCFunction)(void (*)(void))py_paged_attention, METH_FASTCALL, nullptr},
     {"workspace", (PyCFunction)(void (*)(void))py_workspace, METH_FASTCALL, nullptr},
     {"release_workspaces", py_release_workspaces, METH_NOARGS, nullptr},
     {nullptr, nullptr, 0, nullptr},

@@ -276,4 +276,45 @@ SwapPlan plan_swap_w8a16(int64_t M, int64_t K, int64_t N, int force_splits);
 cudaError_t launch_swap_w8a16(const SwapPlan& plan, const UmmaArgs& a, const void* x, int64_t ldx,
                               cudaStream_t stream, const char** why);
 
+// ---- paged key-value cache (kv_cache.cu, paged_attention.cu) ----
+// fp8lin_kv_cache as the kernels take it: checked, strides of the rows in bytes, those of dimensions of one element 0.
+struct CacheView {
+    unsigned char* k;
+    unsigned char* v;
+    float* k_scale;
+    float* v_scale;
+    int64_t num_blocks;
+    int64_t sb, st, sh;            // bytes
+    int64_t ssb, sst, ssh;         // elements
+    int block_size, kv_heads, dim;
+    bool e4m3;
+};
+struct CacheRows {                 // bf16 keys and values in front of (or out of) the cache
+    __nv_bfloat16* k;
+    __nv_bfloat16* v;
+    int64_t kt, kh, vt, vh;        // strides of tokens and heads, elements
+    int64_t rows;
+};
+cudaError_t launch_kv_cache_write(const CacheView& c, const CacheRows& x, const int* slots, int* status, cudaStream_t stream);
+cudaError_t launch_kv_cache_read(const CacheView& c, const CacheRows& y, const int* tables, int64_t ld_tables, int64_t max_pages, const int* cu_seqlens,
+                                 int64_t batch, int* status, cudaStream_t stream);
+struct AttnArgs {
+    CacheView c;
+    const __nv_bfloat16* q;
+    int64_t q_row, q_head;         // elements
+    const int* tables;
+    int64_t ld_tables, max_pages;
+    const int* lens;
+    int batch, heads;
+    float scale;
+    const float* out_scale;        // nullptr: bf16
+    void* out;
+    int64_t ld_out;
+    int* status;
+    int* counters;
+    float* partial;
+};
+size_t paged_attention_scratch(int64_t heads, int64_t kv_heads, int64_t dim, bool e4m3);
+cudaError_t launch_paged_attention(const AttnArgs& a, cudaStream_t stream);
+
 }  // namespace fp8lin

@@ -401,6 +401,13 @@ class RowParallelLinear(LinearBase):
         if self.tp_size == 1:
             return self.apply_linear(x, bias)
         reduce = self.tp_size > 1 and bool(self.reduce_results)
+        if not isinstance(x, torch.Tensor):             # codes of a decode step: a few rows, summed by the all-reduce
+            if self.reduce_results == "scatter":
+                raise ValueError("reduce_results='scatter' takes bfloat16 activations, not codes")
+            y = self.apply_linear(x, bias)
+            if reduce:
+                dist.all_reduce(y, group=self.tp_group)
+            return y
         rows = x.numel() // x.shape[-1] if x.dim() > 0 else 0
         if reduce and (self._use_peer_rs(x, rows) or self._use_peer_reduce(x, rows)):
             try:

@@ -292,3 +292,42 @@ def launch_mlp_w8a8(x: torch.Tensor, w_gate_up_il: torch.Tensor, gate_up_scale_i
     _check_bias(gate_up_bias_il)
     return _lib.host().mlp(x, w_gate_up_il, gate_up_scale_il, gate_up_input_scale, gate_up_bias_il, w_down, down_scale,
                            down_input_scale, down_bias, out)
+
+
+def kv_cache_write(k: torch.Tensor, v: torch.Tensor, slot_mapping: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                   k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None) -> None:
+    """Keys and values of a step's tokens (bfloat16 [N, kv_heads, head_dim], slices of a projection's output as they are) into
+    the pages of a cache: row t goes to slot ``slot_mapping[t]`` (int32; page * block_size + offset), a negative slot is skipped.
+
+    The caches are [num_blocks, block_size, kv_heads, head_dim] with contiguous channels and equal strides, bfloat16, or e4m3
+    codes (float8_e4m3fn, or uint8) with one float32 scale per token and head, ``max(max|x|, 1e-8) / 448``, in ``k_scale`` and
+    ``v_scale`` [num_blocks, block_size, kv_heads].  The slots of one call have to be distinct.  A slot outside the cache is
+    skipped, and the next call on the stream raises ``RuntimeError``."""
+    _lib.host().kv_cache_write(k, v, slot_mapping, k_cache, v_cache, k_scale, v_scale)
+
+
+def kv_cache_read(k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor, cu_seqlens: torch.Tensor, rows: int,
+                  k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None, k_out: torch.Tensor | None = None,
+                  v_out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """The cached tokens of a batch of sequences as bfloat16 (k, v) [rows, kv_heads, head_dim], one sequence behind the other:
+    sequence b gets the rows from ``cu_seqlens[b]`` to ``cu_seqlens[b + 1]`` (int32, on the device), and its first tokens.
+    Rows behind the last sequence (``rows`` may be more, as in a captured graph) are left as they were.  ``block_tables``: int32
+    [batch, pages]; entries behind a sequence's last page may hold anything."""
+    return _lib.host().kv_cache_read(k_cache, v_cache, block_tables, cu_seqlens, rows, k_scale, v_scale, k_out, v_out)
+
+
+def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor, context_lens: torch.Tensor,
+                    scale: float | None = None, k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None,
+                    out_scale: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of one new token per sequence, which is in the cache already, over the first ``context_lens[b]`` (int32) tokens of
+    sequence b: ``softmax(scale * q . K^T) V``, bfloat16 [B, heads, head_dim].  q: bfloat16 [B, heads, head_dim], any strides of whole 16-byte
+    words; ``heads`` a multiple of the cache's kv_heads; ``scale`` None: 1 / sqrt(head_dim).  A context of 0 gives zeros.
+    With ``out_scale`` (one float32 on the device, the input scale of the linear behind the attention) the result is the uint8
+    e4m3 codes that ``quantize_activation`` makes of the bfloat16 one.  ``out``: [B, heads, head_dim] or [B, heads * head_dim]."""
+    return _lib.host().paged_attention(q, k_cache, v_cache, block_tables, context_lens, scale, k_scale, v_scale, out_scale, out)
+
+
+def paged_attention_workspace_bytes(heads: int, kv_heads: int, head_dim: int, dtype: torch.dtype = torch.bfloat16) -> int:
+    """Scratch of ``paged_attention`` on one stream, whatever the batch and its lengths (see ``reserve_workspace``)."""
+    cache = _lib.CACHE_BF16 if dtype == torch.bfloat16 else _lib.CACHE_E4M3
+    return int(_lib.load().fp8lin_paged_attention_workspace_bytes(heads, kv_heads, head_dim, cache))
