@@ -111,6 +111,11 @@ __device__ __forceinline__ uint4 ld_dep_l2(const uint4* p) {
     asm volatile("ld.global.cg.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p) : "memory");
     return r;
 }
+__device__ __forceinline__ float ld_dep_l2(const float* p) {
+    float r;
+    asm volatile("ld.global.cg.f32 %0, [%1];" : "=f"(r) : "l"(p) : "memory");
+    return r;
+}
 __device__ __forceinline__ float2 ld_dep_l2(const float2* p) {
     float2 r;
     asm volatile("ld.global.cg.v2.f32 {%0,%1}, [%2];" : "=f"(r.x), "=f"(r.y) : "l"(p) : "memory");

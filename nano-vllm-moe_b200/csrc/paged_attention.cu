@@ -2,100 +2,795 @@
 //
 //   s_i = scale * q . k_i;   o = sum_i exp(s_i - m) v_i / sum_i exp(s_i - m),   m = max_i s_i
 //
-// in one pass over the tokens: with every token that raises the maximum, the sums so far are scaled by exp(m_old - m_new).
-// One warp per query head, a lane holds eight channels, everything in fp32.
+// in one pass over the tokens: where a block of them raises the maximum, the sums so far are scaled by exp(m_old - m_new).
+// What bounds it is the cache's bytes: 2 D of them (bf16: 4 D) per token and key head, each read once, against 4 D
+// multiplications for each of the group of query heads that share it.
+//
+// Work.  The cached tokens of a key head are cut into tiles of 16; a query group ("segment": one sequence, one key head, up to
+// 8 or 16 of its query heads) is a run of tiles, and all segments one behind the other are one list.  CTAs (one per SM) take equal
+// shares of the list, their warps equal shares of that, so a batch of any lengths keeps every SM busy to the end, and a
+// captured call follows lengths that change: the shares are computed on the device, by every CTA for itself, from the
+// lengths alone.  A segment that several warps share is joined in the CTA; one that several CTAs share by the CTA that
+// comes last, over the pieces in the order of the list (so that the result does not depend on which one comes last).
+//
+// A warp works alone on its tiles: it copies keys and values into a ring of its own with cp.async (16 bytes a lane, rows of any
+// stride, zeros for what lies behind the end), several tiles ahead, and never meets a CTA barrier on the way.
+//
+// Products.  S^T = K Q^T and O^T += V^T P^T with mma.sync.m16n8k16: the tokens, then the channels are the 16 rows, the query heads
+// the 8 columns, so that a group of up to 8 costs half the instructions that queries as rows would, and both products' sums
+// lie with the same columns in the same lanes.  (tcgen05 would take the tiles as they are, but the tensor cores are idle
+// nine cycles out of ten here either way, and its sums would have to go through tensor memory to meet the softmax.)
+// P is split into two numbers of 16 bits, so the weights are good to 2^-16 (bf16) or 2^-21 (f16) instead of 2^-8.
+// e4m3 codes are widened to f16 (exact) behind ldmatrix.  Queries are scaled by a power of two into f16's range; a token's
+// key scale multiplies its scores, its value scale its weight, relative to a power of two near the largest so far.
+#include <atomic>
+
 #include "common.cuh"
 #include "kernels.h"
 
 namespace fp8lin {
+namespace {
 
-constexpr int kAttnThreads = 128;
+constexpr int kTile = 16;                       // tokens
+constexpr float kLog2e = 1.4426950408889634f;
 
-template <bool kE4m3>
-__device__ __forceinline__ void load_row8(const unsigned char* row, int lane, float s, float (&f)[8]) {
-    if (kE4m3) {
-        const long long w = ld_dep(reinterpret_cast<const long long*>(row) + lane);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint32_t h = cvt_e4m3x2_to_f16x2((uint16_t)(w >> (16 * i)));
-            const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&h));
-            f[2 * i] = v.x * s;
-            f[2 * i + 1] = v.y * s;
-        }
+template <bool kE4m3_, int kD_, int kN_, int kWarps_, int kStages_>
+struct Shape {
+    static constexpr bool kE4m3 = kE4m3_;
+    static constexpr int kD = kD_;              // channels in shared memory: head_dim rounded up, zeros behind it
+    static constexpr int kN = kN_;              // groups of 8 query heads
+    static constexpr int kHeads = 8 * kN;
+    static constexpr int kWarps = kWarps_;
+    static constexpr int kStages = kStages_;
+    static constexpr int kThreads = 32 * kWarps;
+    static constexpr int kRow = kD * (kE4m3 ? 1 : 2);                     // bytes of a row
+    static constexpr int kWords = kRow / 16;                              // 16-byte words of a row
+    static constexpr int kRowsPerCopy = kWords >= 32 ? 1 : 32 / kWords;   // rows that a warp's copy instruction takes
+    static constexpr int kCopies = kTile / kRowsPerCopy;
+    static constexpr int kStageBytes = 2 * kTile * kRow + (kE4m3 ? 2 * kTile * 4 : 0);
+    static constexpr int kRing = kWarps * kStages * kStageBytes;
+    static constexpr int kPiece = kHeads * kD;                            // floats of a piece's sums
+    static constexpr int kSmem = kRing > kWarps * kPiece * 4 ? kRing : kWarps * kPiece * 4;
+    static_assert(kWords <= 32, "a row is one copy instruction of a warp at most");
+};
+
+__device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there) {
+    asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy4(uint32_t dst, const void* src, bool there) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(there ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ void copies_end() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kLeft>
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory"); }
+
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ uint32_t transposed(uint32_t a) {              // of an 8 x 8 matrix of 16-bit numbers
+    uint32_t d;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+    return d;
+}
+template <bool kF16>
+__device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    if (kF16)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float exp2_approx(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+// exp2(m - top) for a maximum that may be that of nothing
+__device__ __forceinline__ float weight_of(float m, float top) { return m == -INFINITY ? 0.f : exp2_approx(m - top); }
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t sel) { return __byte_perm(a, 0, sel); }
+
+// Two numbers as hi + lo, each of 16 bits.
+template <bool kF16>
+__device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
+    if (kF16) {
+        hi = pack_f16x2(x, y);
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+        lo = pack_f16x2(x - f.x, y - f.y);
     } else {
-        const uint4 w = ld_dep(reinterpret_cast<const uint4*>(row) + lane);
-        const uint32_t v[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) { f[2 * i] = bf16_lo(v[i]); f[2 * i + 1] = bf16_hi(v[i]); }
+        hi = pack_bf16x2(x, y);
+        lo = pack_bf16x2(x - bf16_lo(hi), y - bf16_hi(hi));
     }
 }
 
-template <bool kE4m3>
-__global__ void __launch_bounds__(kAttnThreads)
-paged_attention_kernel(AttnArgs a) {
+// Tiles of a sequence; an empty one has one as well, of nothing, so that its zeros are written like any result.
+__device__ __forceinline__ int tokens_of(const AttnArgs& a, int64_t b, int64_t most) {
+    const int len = ld_dep(a.lens + b);
+    return len < 0 ? 0 : (int64_t)len > most ? (int)most : len;
+}
+__device__ __forceinline__ int tiles_of(int len) { return len > kTile ? (int)(((unsigned)len + kTile - 1) / kTile) : 1; }
+
+// Whose share of `total` tiles among `parts` a tile is in: part p has [total p / parts, total (p + 1) / parts).
+__device__ __forceinline__ int64_t share_begin(int64_t total, int parts, int64_t p) { return total * p / parts; }
+__device__ __forceinline__ int share_of(int64_t total, int parts, int64_t tile) { return (int)(((tile + 1) * parts - 1) / total); }
+
+struct Piece {                  // part of a segment
+    int64_t tile0;              // the segment's first tile in the list, -1: none
+    int tiles, b, hc;           // its tiles, sequence, key head and part of its query heads
+};
+
+// Four channels of a query head, the finished sums.
+__device__ __forceinline__ void store4(const AttnArgs& a, int b, int head, int d, float4 v) {
+    if (d >= a.c.dim) return;
+    const int64_t at = (int64_t)b * a.ld_out + (int64_t)head * a.c.dim + d;
+    const uint2 w = {pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w)};
+    if (!a.out_scale) {
+        *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.out) + at) = w;
+        return;
+    }
+    const ExactDiv div(fmaxf(ld_dep(a.out_scale), 1e-12f));
+    const uint32_t lo = cvt_e4m3x2(div(bf16_lo(w.x)), div(bf16_hi(w.x))), hi = cvt_e4m3x2(div(bf16_lo(w.y)), div(bf16_hi(w.y)));
+    *reinterpret_cast<uint32_t*>(static_cast<unsigned char*>(a.out) + at) = lo | (hi << 16);
+}
+// ... and two, from the fragments of a warp that had the whole segment
+__device__ __forceinline__ void store2(const AttnArgs& a, int b, int head, int d, uint32_t w) {
+    const int64_t at = (int64_t)b * a.ld_out + (int64_t)head * a.c.dim + d;
+    if (!a.out_scale) {
+        *reinterpret_cast<uint32_t*>(static_cast<__nv_bfloat16*>(a.out) + at) = w;
+        return;
+    }
+    const ExactDiv div(fmaxf(ld_dep(a.out_scale), 1e-12f));
+    *reinterpret_cast<uint16_t*>(static_cast<unsigned char*>(a.out) + at) = cvt_e4m3x2(div(bf16_lo(w)), div(bf16_hi(w)));
+}
+
+// Scratch: the sums of a warp's first piece where it went on to another segment, then two pieces per CTA with their statistics.
+template <class S>
+__host__ __device__ constexpr size_t scratch_floats(int ctas) {
+    return (size_t)ctas * S::kWarps * S::kPiece + (size_t)ctas * 2 * (S::kPiece + 2 * S::kHeads);
+}
+
+template <class S>
+__global__ void __launch_bounds__(S::kThreads, 1)
+paged_attention_kernel(AttnArgs a, int group, int parts) {
+    constexpr bool kE4m3 = S::kE4m3;
+    constexpr int kD = S::kD, kN = S::kN, kHeads = S::kHeads, kWarps = S::kWarps, kStages = S::kStages, kRow = S::kRow, kPiece = S::kPiece;
+    extern __shared__ __align__(1024) unsigned char ring[];
+    __shared__ int64_t s_scan[kWarps], s_base[kWarps];
+    __shared__ int s_b[kWarps];
+    __shared__ Piece s_piece[2 * kWarps];
+    __shared__ float s_m[2 * kWarps][kHeads], s_l[2 * kWarps][kHeads];
+    __shared__ uint32_t s_run[2 * kWarps];      // the pieces of a run (bits), pieces of one segment
+    __shared__ int s_runs, s_open[2], s_last[2];
+
     pdl_launch_dependents();
     pdl_wait();
-    const int lane = threadIdx.x & 31;
-    const int64_t row = (int64_t)blockIdx.x * (kAttnThreads / 32) + (threadIdx.x >> 5);
-    const int64_t b = row / a.heads;
-    if (b >= a.batch) return;
-    const int head = (int)(row - b * a.heads);
-    const int kvh = head / (a.heads / a.c.kv_heads);
-    const bool mine = lane * 8 < a.c.dim;
-    float q[8] = {}, o[8] = {}, m = -INFINITY, l = 0.f;
-    if (mine) load_row8<false>(reinterpret_cast<const unsigned char*>(a.q + b * a.q_row + head * a.q_head), lane, 1.f, q);
-    int len = ld_dep(a.lens + b);
-    if ((int64_t)len > a.max_pages * a.c.block_size) {
-        len = (int)(a.max_pages * a.c.block_size);
-        if (lane == 0) report_status(a.status, kDevBadPage);
-    }
-    for (int t = 0; t < len; ++t) {
-        const int i = t / a.c.block_size, off = t - i * a.c.block_size;
-        const int64_t page = ld_dep(a.tables + b * a.ld_tables + i);
-        if (page < 0 || page >= a.c.num_blocks) {
-            if (lane == 0) report_status(a.status, kDevBadPage);
-            continue;
-        }
-        const int64_t at = page * a.c.sb + off * a.c.st + kvh * a.c.sh, scale_at = page * a.c.ssb + off * a.c.sst + kvh * a.c.ssh;
-        float k[8] = {}, v[8] = {}, s = 0.f;
-        if (mine) {
-            load_row8<kE4m3>(a.c.k + at, lane, kE4m3 ? ld_dep(a.c.k_scale + scale_at) : 1.f, k);
-            load_row8<kE4m3>(a.c.v + at, lane, kE4m3 ? ld_dep(a.c.v_scale + scale_at) : 1.f, v);
-        }
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int segments = a.c.kv_heads * parts;                                   // per sequence
+    const int64_t most64 = a.max_pages * a.c.block_size, most = most64 < 0x7fffffff ? most64 : 0x7fffffff;
+
+    // ---- shares -----------------------------------------------------------------------------------------------------
+    auto block_scan = [&](int64_t v, int64_t& before, int64_t& all) {             // exclusive sum over the threads, and all of it
+        int64_t x = v;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) s = fmaf(q[e], k[e], s);
-        for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-        s *= a.scale;
-        const float top = fmaxf(m, s);
-        const float old = m == -INFINITY ? 0.f : expf(m - top), p = expf(s - top);
-        m = top;
-        l = l * old + p;
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= o) x += y;
+        }
+        if (lane == 31) s_scan[warp] = x;
+        __syncthreads();
+        before = x - v;
+        all = 0;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) o[e] = o[e] * old + p * v[e];
+        for (int w = 0; w < kWarps; ++w) {
+            if (w < warp) before += s_scan[w];
+            all += s_scan[w];
+        }
+        __syncthreads();
+    };
+    if (tid < 2) s_open[tid] = -1;
+    const bool once = a.batch <= S::kThreads;
+    int64_t total = 0, before = 0;
+    int my_tiles = 0;
+    auto look = [&](int b) {
+        if (b >= a.batch) return 0;
+        if (blockIdx.x == 0 && (int64_t)ld_dep(a.lens + b) > most) report_status(a.status, kDevBadPage);
+        return tiles_of(tokens_of(a, b, most));
+    };
+    if (once) {
+        my_tiles = look(tid);
+        block_scan((int64_t)my_tiles * segments, before, total);
+    } else {
+        int64_t sum = 0, unused;
+        for (int b = tid; b < a.batch; b += S::kThreads) sum += (int64_t)look(b) * segments;
+        block_scan(sum, unused, total);
     }
-    if (!mine) return;
-    const float inv = len > 0 ? 1.f / l : 0.f;
-    uint4 w;
-    w.x = pack_bf16x2(o[0] * inv, o[1] * inv);
-    w.y = pack_bf16x2(o[2] * inv, o[3] * inv);
-    w.z = pack_bf16x2(o[4] * inv, o[5] * inv);
-    w.w = pack_bf16x2(o[6] * inv, o[7] * inv);
-    const int64_t out = b * a.ld_out + (int64_t)head * a.c.dim + lane * 8;
-    if (a.out_scale) *reinterpret_cast<uint2*>(static_cast<unsigned char*>(a.out) + out) = quant8_e4m3(w, ExactDiv(fmaxf(ld_dep(a.out_scale), 1e-12f)));
-    else *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.out) + out) = w;
+    // one tile per warp at least
+    const int64_t wanted = (total + kWarps - 1) / kWarps;
+    const int ctas = wanted < gridDim.x ? (int)wanted : (int)gridDim.x;
+    if ((int)blockIdx.x >= ctas) return;
+    const int64_t cta0 = share_begin(total, ctas, blockIdx.x), cta1 = share_begin(total, ctas, blockIdx.x + 1);
+    auto place = [&](int b, int tiles, int64_t at) {                               // which warps begin in sequence b's tiles
+        const int64_t end = at + (int64_t)tiles * segments;
+        if (tiles == 0 || end <= cta0 || at >= cta1) return;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            const int64_t begin = cta0 + share_begin(cta1 - cta0, kWarps, w);
+            if (begin >= at && begin < end) { s_b[w] = b; s_base[w] = at; }
+        }
+    };
+    if (once) {
+        place(tid, my_tiles, before);
+    } else {
+        int64_t base = 0;
+        for (int b0 = 0; b0 < a.batch && base < cta1; b0 += S::kThreads) {
+            const int b = b0 + tid, tiles = b < a.batch ? tiles_of(tokens_of(a, b, most)) : 0;
+            int64_t all;
+            block_scan((int64_t)tiles * segments, before, all);
+            place(b, tiles, base + before);
+            base += all;
+        }
+    }
+    __syncthreads();
+    const int64_t begin = cta0 + share_begin(cta1 - cta0, kWarps, warp);
+    const int64_t todo = cta0 + share_begin(cta1 - cta0, kWarps, warp + 1) - begin;
+
+    // ---- a warp's tiles -----------------------------------------------------------------------------------------------
+    unsigned char* const my_ring = ring + warp * (kStages * S::kStageBytes);
+    const int row_bytes = a.c.dim * (kE4m3 ? 1 : 2);
+    const bool paged16 = a.c.block_size % kTile == 0;
+    const int g = lane >> 2, t4 = lane & 3;
+
+    struct Place { int b, hc, t, len, tiles; } in, at;              // of the next tile to copy, and to work on
+    int next_len = 0, page = 0, page_at = 0, page_off = 0;
+    auto next_page = [&] {                                          // of tile `in`, asked for one tile early
+        if (paged16 && in.t * kTile < in.len) page = ld_dep(a.tables + (int64_t)in.b * a.ld_tables + page_at);
+    };
+    if (todo > 0) {
+        const int b = s_b[warp];
+        const int64_t inside = begin - s_base[warp];
+        in.b = b;
+        in.len = tokens_of(a, b, most);
+        in.tiles = tiles_of(in.len);
+        in.hc = (int)(inside / in.tiles);
+        in.t = (int)(inside - (int64_t)in.hc * in.tiles);
+        at = in;
+        page_at = in.t * kTile / a.c.block_size;
+        page_off = in.t * kTile - page_at * a.c.block_size;
+        next_page();
+        if (b + 1 < a.batch) next_len = tokens_of(a, b + 1, most);
+    }
+    // copies: lane -> word `word` of the rows copy_row + j * kRowsPerCopy
+    const int copy_row = lane / S::kWords, word = lane % S::kWords;
+    auto swizzle = [](int r, int w) { return S::kWords >= 8 ? (w & ~7) | ((w ^ r) & 7) : (w ^ (r >> 1)) & 3; };
+    const uint32_t copy_dst = copy_row * kRow + swizzle(copy_row, word) * 16;
+    auto copy_tile = [&](int stage) {
+        const uint32_t ks = smem_addr(my_ring) + stage * S::kStageBytes, vs = ks + kTile * kRow;
+        const int head = in.hc / parts, rows = in.len - in.t * kTile;             // rows that exist: at least 16, but at a sequence's end
+        const int64_t v_less_k = a.c.v - a.c.k;
+        const bool word_there = word * 16 < row_bytes;
+        if (paged16) {
+            bool there = rows > 0;
+            int64_t p = page;
+            if (there && (p < 0 || p >= a.c.num_blocks)) {
+                there = false;
+                if (lane == 0) report_status(a.status, kDevBadPage);
+            }
+            if (!there) p = 0;
+            const unsigned char* src = a.c.k + p * a.c.sb + (there ? page_off : 0) * a.c.st + head * a.c.sh;
+#pragma unroll
+            for (int j = 0; j < S::kCopies; ++j) {
+                const int r = copy_row + j * S::kRowsPerCopy;
+                const bool ok = there && r < rows && word_there;
+                const unsigned char* row = ok ? src + r * a.c.st + word * 16 : a.c.k;
+                const uint32_t dst = j * S::kRowsPerCopy * kRow + (copy_dst ^ (S::kWords >= 8 ? ((j * S::kRowsPerCopy) & 7) * 16 : 0));
+                copy16(ks + dst, row, ok);
+                copy16(vs + dst, row + v_less_k, ok);
+            }
+            if (kE4m3) {
+                const int r = lane & 15;
+                const bool ok = there && r < rows;
+                const float* s = (lane < 16 ? a.c.k_scale : a.c.v_scale) + (ok ? p * a.c.ssb + (int64_t)(page_off + r) * a.c.sst + head * a.c.ssh : 0);
+                copy4(vs + kTile * kRow + lane * 4, s, ok);
+            }
+            page_off += kTile;
+            if (page_off == a.c.block_size) { page_off = 0; ++page_at; }
+        } else {                                                                  // every row has a page of its own
+            const int r16 = lane & 15, token = in.t * kTile + r16;
+            bool there = r16 < rows;
+            int64_t p = 0, off = 0;
+            if (there) {
+                const int i = token / a.c.block_size;
+                off = token - (int64_t)i * a.c.block_size;
+                p = ld_dep(a.tables + (int64_t)in.b * a.ld_tables + i);
+                if (p < 0 || p >= a.c.num_blocks) {
+                    there = false;
+                    report_status(a.status, kDevBadPage);
+                }
+            }
+            const long long mine = there ? p * a.c.sb + off * a.c.st + head * a.c.sh : -1;
+#pragma unroll
+            for (int j = 0; j < S::kCopies; ++j) {
+                const long long from = __shfl_sync(0xffffffffu, mine, copy_row + j * S::kRowsPerCopy);
+                const bool ok = from >= 0 && word_there;
+                const unsigned char* row = ok ? a.c.k + from + word * 16 : a.c.k;
+                const uint32_t dst = j * S::kRowsPerCopy * kRow + (copy_dst ^ (S::kWords >= 8 ? ((j * S::kRowsPerCopy) & 7) * 16 : 0));
+                copy16(ks + dst, row, ok);
+                copy16(vs + dst, row + v_less_k, ok);
+            }
+            if (kE4m3) {
+                const float* s = (lane < 16 ? a.c.k_scale : a.c.v_scale) + (there ? p * a.c.ssb + off * a.c.sst + head * a.c.ssh : 0);
+                copy4(vs + kTile * kRow + lane * 4, s, there);
+            }
+        }
+        // on to the next tile
+        if (++in.t == in.tiles) {
+            in.t = 0;
+            page_at = page_off = 0;
+            if (++in.hc == segments) {
+                in.hc = 0;
+                ++in.b;
+                in.len = next_len;
+                in.tiles = tiles_of(in.len);
+                if (in.b + 1 < a.batch) next_len = tokens_of(a, in.b + 1, most);
+            }
+        }
+    };
+
+    uint32_t q[kD / 16][kN][2];
+    float o[kD / 16][kN][4], m[kN][2], l[kN][2], to_score[kN][2];
+    int value_exp = 15;                                                            // exponent field that the values' scales are relative to
+    auto begin_segment = [&] {
+        const int part = at.hc % parts, head0 = at.hc / parts * group + part * kHeads, heads = min(kHeads, group - part * kHeads);
+        value_exp = 15;
+#pragma unroll
+        for (int n = 0; n < kN; ++n) {
+            const __nv_bfloat16* row = a.q + (int64_t)at.b * a.q_row + (int64_t)(head0 + n * 8 + g) * a.q_head;
+            const bool real = n * 8 + g < heads;
+            uint32_t top = 0;
+#pragma unroll
+            for (int s = 0; s < kD / 16; ++s) {
+                uint32_t x = 0, y = 0;
+                if (real && s * 16 < a.c.dim) {
+                    if (kE4m3) {
+                        const long long w = ld_dep(reinterpret_cast<const long long*>(row + s * 16 + t4 * 4));
+                        x = (uint32_t)w;
+                        y = (uint32_t)(w >> 32);
+                    } else {
+                        x = ld_dep(reinterpret_cast<const int*>(row + s * 16 + t4 * 2));
+                        y = ld_dep(reinterpret_cast<const int*>(row + s * 16 + 8 + t4 * 2));
+                    }
+                }
+                q[s][n][0] = x;
+                q[s][n][1] = y;
+                if (kE4m3) top = __vmaxu2(top, __vmaxu2(x & 0x7fff7fffu, y & 0x7fff7fffu));
+            }
+            const float base = a.scale * kLog2e;
+            if (kE4m3) {
+                // the largest channel to 2^14 .. 2^15: f16 holds those down to 2^-29 of it with all of bf16's bits
+                top = max(top & 0xffffu, top >> 16);
+                top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                const int e = (int)(top >> 7), up = e == 255 ? 0 : 14 + 127 - (e == 0 ? 1 : e);
+#pragma unroll
+                for (int s = 0; s < kD / 16; ++s)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const uint32_t w = q[s][n][i];
+                        q[s][n][i] = pack_f16x2(ldexpf(bf16_lo(w), up), ldexpf(bf16_hi(w), up));
+                    }
+#pragma unroll
+                for (int i = 0; i < 2; ++i) to_score[n][i] = ldexpf(base, -__shfl_sync(0xffffffffu, up, (2 * t4 + i) * 4));
+            } else {
+                to_score[n][0] = to_score[n][1] = base;
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) { m[n][i] = -INFINITY; l[n][i] = 0.f; }
+#pragma unroll
+            for (int c = 0; c < kD / 16; ++c)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[c][n][i] = 0.f;
+        }
+    };
+
+    const int mi = lane >> 3, lr = lane & 7;                                       // ldmatrix: this lane's matrix and row
+    auto work_on = [&](int stage) {
+        const uint32_t ks = smem_addr(my_ring) + stage * S::kStageBytes, vs = ks + kTile * kRow;
+        float s[kN][4];
+#pragma unroll
+        for (int n = 0; n < kN; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[n][i] = 0.f;
+        // scores: rows of the A operand are tokens
+        {
+            const int r = lr + (mi & 1) * 8;
+#pragma unroll
+            for (int c = 0; c < kD / 16; c += kE4m3 ? 2 : 1) {
+                uint32_t f[4];
+                const int w = (kE4m3 ? c : 2 * c) + (mi >> 1);
+                ldmatrix4(f, ks + r * kRow + swizzle(r, w) * 16);
+                if (kE4m3) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const uint32_t x = f[2 * h], y = f[2 * h + 1];
+                        const uint32_t a0 = cvt_e4m3x2_to_f16x2((uint16_t)x), a2 = cvt_e4m3x2_to_f16x2((uint16_t)(x >> 16));
+                        const uint32_t a1 = cvt_e4m3x2_to_f16x2((uint16_t)y), a3 = cvt_e4m3x2_to_f16x2((uint16_t)(y >> 16));
+#pragma unroll
+                        for (int n = 0; n < kN; ++n) mma<true>(s[n], a0, a1, a2, a3, q[c + h][n][0], q[c + h][n][1]);
+                    }
+                } else {
+#pragma unroll
+                    for (int n = 0; n < kN; ++n) mma<false>(s[n], f[0], f[1], f[2], f[3], q[c][n][0], q[c][n][1]);
+                }
+            }
+        }
+        float k_scale[2], v_scale[2];                                              // of tokens g and g + 8
+        if (kE4m3) {
+            const float* sc = reinterpret_cast<const float*>(my_ring + stage * S::kStageBytes + 2 * kTile * kRow);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) { k_scale[h] = sc[g + 8 * h]; v_scale[h] = sc[kTile + g + 8 * h]; }
+        }
+        const int rows = at.len - at.t * kTile;
+        float top[kN][2];
+        bool raised = false;
+#pragma unroll
+        for (int n = 0; n < kN; ++n) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (kE4m3) s[n][i] *= k_scale[i >> 1];
+                s[n][i] *= to_score[n][i & 1];
+                if (rows < kTile && g + 8 * (i >> 1) >= rows) s[n][i] = -INFINITY;
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                float x = fmaxf(s[n][i], s[n][2 + i]);
+                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+                top[n][i] = fmaxf(m[n][i], x);
+                raised |= top[n][i] != m[n][i];
+            }
+        }
+        int exp_now = value_exp;
+        if (kE4m3) {
+            const uint32_t e = __reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(fabsf(v_scale[0]), fabsf(v_scale[1])))) >> 23;
+            exp_now = max(value_exp, (int)e);
+            raised |= exp_now != value_exp;
+        }
+        if (__any_sync(0xffffffffu, raised)) {
+            const float down = kE4m3 ? exp2_approx((float)(value_exp - exp_now)) : 1.f;
+#pragma unroll
+            for (int n = 0; n < kN; ++n)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const float f = weight_of(m[n][i], top[n][i]);
+                    m[n][i] = top[n][i];
+                    l[n][i] *= f;
+#pragma unroll
+                    for (int c = 0; c < kD / 16; ++c) { o[c][n][i] *= f * down; o[c][n][2 + i] *= f * down; }
+                }
+            value_exp = exp_now;
+        }
+        uint32_t hi[kN][2], lo[kN][2];
+        const float up = kE4m3 ? __uint_as_float((uint32_t)(268 - value_exp) << 23) : 1.f;    // 2^(14 - (value_exp - 127))
+#pragma unroll
+        for (int n = 0; n < kN; ++n)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                float p[2];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    p[i] = exp2_approx(s[n][2 * h + i] - (m[n][i] == -INFINITY ? 0.f : m[n][i]));
+                    l[n][i] += p[i];
+                    if (kE4m3) p[i] *= v_scale[h] * up;
+                }
+                split2<kE4m3>(p[0], p[1], hi[n][h], lo[n][h]);
+                hi[n][h] = transposed(hi[n][h]);
+                lo[n][h] = transposed(lo[n][h]);
+            }
+        // values: rows of the A operand are channels
+#pragma unroll
+        for (int c = 0; c < kD / 16; c += kE4m3 ? 2 : 1) {
+            uint32_t f[4];
+            if (kE4m3) {
+                // a lane's word holds channels 2g and 2g + 1 of two tokens: the first are row g, the second row g + 8
+                const int r = lr + (mi & 1) * 8, w = c + (mi >> 1);
+                ldmatrix4_trans(f, vs + r * kRow + swizzle(r, w) * 16);
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const uint32_t x = prmt(f[2 * h], 0x3120), y = prmt(f[2 * h + 1], 0x3120);
+                    const uint32_t a0 = cvt_e4m3x2_to_f16x2((uint16_t)x), a1 = cvt_e4m3x2_to_f16x2((uint16_t)(x >> 16));
+                    const uint32_t a2 = cvt_e4m3x2_to_f16x2((uint16_t)y), a3 = cvt_e4m3x2_to_f16x2((uint16_t)(y >> 16));
+#pragma unroll
+                    for (int n = 0; n < kN; ++n) {
+                        mma<true>(o[c + h][n], a0, a1, a2, a3, hi[n][0], hi[n][1]);
+                        mma<true>(o[c + h][n], a0, a1, a2, a3, lo[n][0], lo[n][1]);
+                    }
+                }
+            } else {
+                const int r = lr + (mi >> 1) * 8, w = 2 * c + (mi & 1);
+                ldmatrix4_trans(f, vs + r * kRow + swizzle(r, w) * 16);
+#pragma unroll
+                for (int n = 0; n < kN; ++n) {
+                    mma<false>(o[c][n], f[0], f[1], f[2], f[3], hi[n][0], hi[n][1]);
+                    mma<false>(o[c][n], f[0], f[1], f[2], f[3], lo[n][0], lo[n][1]);
+                }
+            }
+        }
+    };
+    // the channels of o[c][.][0..1] and o[c][.][2..3]
+    auto channel = [&](int c, int half) { return kE4m3 ? c * 16 + 2 * g + half : c * 16 + g + 8 * half; };
+    // A piece's sums with their statistics; `last`: the warp's last piece, kept in shared memory, else in scratch.
+    auto keep_piece = [&](bool last, float* sums) {
+        const int e = 2 * warp + last;
+#pragma unroll
+        for (int n = 0; n < kN; ++n)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int col = n * 8 + 2 * t4 + i;
+                if (g == 0) { s_m[e][col] = m[n][i]; s_l[e][col] = l[n][i]; }
+#pragma unroll
+                for (int c = 0; c < kD / 16; ++c) {
+                    sums[col * kD + channel(c, 0)] = o[c][n][i];
+                    sums[col * kD + channel(c, 1)] = o[c][n][2 + i];
+                }
+            }
+    };
+    float* const early = a.partial + ((int64_t)blockIdx.x * kWarps + warp) * kPiece;
+    bool kept = false;
+    if (lane < 2) s_piece[2 * warp + lane].tile0 = -1;
+    __syncwarp();
+    int to = 0, from = 0;                                                          // stages: of the next copy, of the next tile's work
+    for (int64_t i = 1 - kStages; i < todo; ++i) {
+        if (i >= 0) {
+            copies_wait<kStages - 2>();
+            __syncwarp();
+        }
+        const int64_t ahead = i + kStages - 1;
+        if (ahead < todo) {
+            copy_tile(to);
+            to = to + 1 == kStages ? 0 : to + 1;
+            if (ahead + 1 < todo) next_page();
+        }
+        copies_end();
+        if (i < 0) continue;
+        if (i == 0 || at.t == 0) begin_segment();
+        work_on(from);
+        from = from + 1 == kStages ? 0 : from + 1;
+        const bool ends = at.t + 1 == at.tiles, last = i + 1 == todo;
+        if (ends || last) {
+            const float back = kE4m3 ? __uint_as_float((uint32_t)(value_exp - 14) << 23) : 1.f;
+#pragma unroll
+            for (int n = 0; n < kN; ++n)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    l[n][j] += __shfl_xor_sync(0xffffffffu, l[n][j], 4);
+                    l[n][j] += __shfl_xor_sync(0xffffffffu, l[n][j], 8);
+                    l[n][j] += __shfl_xor_sync(0xffffffffu, l[n][j], 16);
+                    if (kE4m3)
+#pragma unroll
+                        for (int c = 0; c < kD / 16; ++c) { o[c][n][j] *= back; o[c][n][2 + j] *= back; }
+                }
+            if (ends && i >= at.t) {                                               // the whole segment was this warp's
+                const int part = at.hc % parts, head0 = at.hc / parts * group + part * kHeads, heads = min(kHeads, group - part * kHeads);
+#pragma unroll
+                for (int n = 0; n < kN; ++n) {
+                    float inv[2];
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) inv[j] = at.len > 0 ? __fdiv_rn(1.f, l[n][j]) : 0.f;
+#pragma unroll
+                    for (int c = 0; c < kD / 16; ++c) {
+                        if (c * 16 >= a.c.dim) continue;
+                        if (kE4m3) {
+#pragma unroll
+                            for (int j = 0; j < 2; ++j) {
+                                const int col = n * 8 + 2 * t4 + j;
+                                if (col < heads) store2(a, at.b, head0 + col, channel(c, 0), pack_bf16x2(o[c][n][j] * inv[j], o[c][n][2 + j] * inv[j]));
+                            }
+                        } else {
+                            const int col = n * 8 + g;
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {                          // lanes of a head side by side: its channels 2 t4, 2 t4 + 1
+                                const uint32_t w = transposed(pack_bf16x2(o[c][n][2 * h] * inv[0], o[c][n][2 * h + 1] * inv[1]));
+                                if (col < heads) store2(a, at.b, head0 + col, c * 16 + 8 * h + 2 * t4, w);
+                            }
+                        }
+                    }
+                }
+            } else {
+                if (lane == 0) s_piece[2 * warp + last] = {begin + i - at.t, at.tiles, at.b, at.hc};
+                if (last) kept = true;                                             // stays in registers until the rings are done with
+                else keep_piece(false, early);
+            }
+        }
+        if (++at.t == at.tiles) {
+            at.t = 0;
+            if (++at.hc == segments) {
+                at.hc = 0;
+                ++at.b;
+                if (i + 1 < todo) {
+                    at.len = tokens_of(a, at.b, most);
+                    at.tiles = tiles_of(at.len);
+                }
+            }
+        }
+    }
+
+    // ---- pieces of a segment in this CTA ------------------------------------------------------------------------------
+    copies_wait<0>();
+    __syncthreads();
+    float* const sums = reinterpret_cast<float*>(ring);                            // [warp][head][channel], over the rings
+    if (kept) keep_piece(true, sums + warp * kPiece);
+    if (warp == 0) {
+        const int64_t seg = lane < 2 * kWarps ? s_piece[lane].tile0 : -1;
+        const uint32_t there = __ballot_sync(0xffffffffu, seg >= 0);
+        const uint32_t below = there & ((1u << lane) - 1);
+        const int64_t prev = __shfl_sync(0xffffffffu, seg, below ? 31 - __clz(below) : lane);
+        const bool first = seg >= 0 && (below == 0 || prev != seg);
+        const uint32_t firsts = __ballot_sync(0xffffffffu, first);
+        if (first) {
+            const uint32_t above = firsts & ~((2u << lane) - 1);
+            const int run = __popc(firsts & ((1u << lane) - 1));
+            s_run[run] = there & ~((1u << lane) - 1) & (above ? (1u << (__ffs(above) - 1)) - 1 : 0xffffffffu);
+            const Piece p = s_piece[lane];
+            if (p.tile0 < cta0) s_open[0] = run;
+            else if (p.tile0 + p.tiles > cta1) s_open[1] = run;
+        }
+        if (lane == 0) s_runs = __popc(firsts);
+    }
+    __syncthreads();
+    constexpr int kUnits = kPiece / 4;                                             // four channels of one head
+    float* const pieces = a.partial + (int64_t)gridDim.x * kWarps * kPiece;         // [CTA][2][sums | m | l]
+    constexpr int kOut = kPiece + 2 * kHeads;
+    const int runs = s_runs;
+    for (int x = tid; x < runs * kUnits; x += S::kThreads) {
+        const int run = x / kUnits, unit = x - run * kUnits, col = unit / (kD / 4), d = unit % (kD / 4) * 4;
+        const uint32_t members = s_run[run];
+        const Piece p = s_piece[__ffs(members) - 1];
+        float top = -INFINITY, total_l = 0.f;
+        for (uint32_t left = members; left; left &= left - 1) top = fmaxf(top, s_m[__ffs(left) - 1][col]);
+        float4 v = {0.f, 0.f, 0.f, 0.f};
+        for (uint32_t left = members; left; left &= left - 1) {
+            const int e = __ffs(left) - 1;
+            const float f = weight_of(s_m[e][col], top);
+            const float* from = (e & 1) ? sums + (e >> 1) * kPiece : a.partial + ((int64_t)blockIdx.x * kWarps + (e >> 1)) * kPiece;
+            const float4 w = *reinterpret_cast<const float4*>(from + col * kD + d);
+            total_l += f * s_l[e][col];
+            v.x += f * w.x; v.y += f * w.y; v.z += f * w.z; v.w += f * w.w;
+        }
+        const int part = p.hc % parts, head = p.hc / parts * group + part * kHeads + col;
+        if (run == s_open[0] || run == s_open[1]) {
+            float* out = pieces + ((int64_t)blockIdx.x * 2 + (run == s_open[1])) * kOut;
+            *reinterpret_cast<float4*>(out + col * kD + d) = v;
+            if (d == 0) { out[kPiece + col] = top; out[kPiece + kHeads + col] = total_l; }
+        } else if (part * kHeads + col < group) {
+            const float inv = __fdiv_rn(1.f, total_l);
+            store4(a, p.b, head, d, {v.x * inv, v.y * inv, v.z * inv, v.w * inv});
+        }
+    }
+
+    // ---- segments that other CTAs have pieces of: the last one to come joins them --------------------------------------
+    if (s_open[0] < 0 && s_open[1] < 0) return;
+    __threadfence();
+    __syncthreads();
+    if (tid < 2) {
+        bool last = false;
+        if (s_open[tid] >= 0) {
+            const Piece p = s_piece[__ffs(s_run[s_open[tid]]) - 1];
+            const int c0 = share_of(total, ctas, p.tile0), c1 = share_of(total, ctas, p.tile0 + p.tiles - 1);
+            __threadfence();
+            last = atomicAdd(a.counters + c0, 1) == c1 - c0;
+            if (last) a.counters[c0] = 0;                                          // for the next call
+            __threadfence();
+        }
+        s_last[tid] = last;
+    }
+    __syncthreads();
+#pragma unroll 1
+    for (int w = 0; w < 2; ++w) {
+        if (!s_last[w]) continue;
+        const Piece p = s_piece[__ffs(s_run[s_open[w]]) - 1];
+        const int c0 = share_of(total, ctas, p.tile0), c1 = share_of(total, ctas, p.tile0 + p.tiles - 1);
+        const int part = p.hc % parts, head0 = p.hc / parts * group + part * kHeads;
+        for (int unit = tid; unit < kUnits; unit += S::kThreads) {
+            const int col = unit / (kD / 4), d = unit % (kD / 4) * 4;
+            float top = -INFINITY, total_l = 0.f;
+            float4 v = {0.f, 0.f, 0.f, 0.f};
+            constexpr int kAtOnce = 8;
+            for (int c = c0; c <= c1; c += kAtOnce) {
+                float4 x[kAtOnce];
+                float xm[kAtOnce], xl[kAtOnce], now = top;
+#pragma unroll
+                for (int j = 0; j < kAtOnce; ++j) {
+                    xm[j] = -INFINITY;
+                    xl[j] = 0.f;
+                    x[j] = {0.f, 0.f, 0.f, 0.f};
+                    if (c + j <= c1) {
+                        const float* from = pieces + ((int64_t)(c + j) * 2 + (c + j == c0)) * kOut;
+                        const uint4 raw = ld_dep_l2(reinterpret_cast<const uint4*>(from + col * kD + d));
+                        x[j] = {__uint_as_float(raw.x), __uint_as_float(raw.y), __uint_as_float(raw.z), __uint_as_float(raw.w)};
+                        xm[j] = ld_dep_l2(from + kPiece + col);
+                        xl[j] = ld_dep_l2(from + kPiece + kHeads + col);
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < kAtOnce; ++j) now = fmaxf(now, xm[j]);
+                const float f0 = weight_of(top, now);
+                total_l *= f0;
+                v.x *= f0; v.y *= f0; v.z *= f0; v.w *= f0;
+#pragma unroll
+                for (int j = 0; j < kAtOnce; ++j) {
+                    const float f = weight_of(xm[j], now);
+                    total_l += f * xl[j];
+                    v.x += f * x[j].x; v.y += f * x[j].y; v.z += f * x[j].z; v.w += f * x[j].w;
+                }
+                top = now;
+            }
+            if (part * kHeads + col < group) {
+                const float inv = __fdiv_rn(1.f, total_l);
+                store4(a, p.b, head0 + col, d, {v.x * inv, v.y * inv, v.z * inv, v.w * inv});
+            }
+        }
+    }
 }
 
-size_t paged_attention_scratch(int64_t, int64_t, int64_t, bool) { return 0; }
-
-cudaError_t launch_paged_attention(const AttnArgs& a, cudaStream_t stream) {
+template <class S>
+cudaError_t launch(const AttnArgs& a, int group, int parts, cudaStream_t stream) {
+    auto kern = paged_attention_kernel<S>;
+    static std::atomic<uint64_t> ready{0};              // devices whose copy of the kernel may take this much shared memory
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev >= 64 || !(ready.load(std::memory_order_acquire) >> dev & 1)) {
+        e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
+        if (e != cudaSuccess) return e;
+        if (dev < 64) ready.fetch_or(1ull << dev, std::memory_order_release);
+    }
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(((int64_t)a.batch * a.heads + kAttnThreads / 32 - 1) / (kAttnThreads / 32)));
-    cfg.blockDim = dim3(kAttnThreads);
+    cfg.gridDim = dim3((unsigned)sm_count());
+    cfg.blockDim = dim3(S::kThreads);
+    cfg.dynamicSmemBytes = S::kSmem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     cfg.numAttrs = pdl_attribute(attr);
     cfg.attrs = attr;
-    return counted(cudaLaunchKernelEx(&cfg, a.c.e4m3 ? paged_attention_kernel<true> : paged_attention_kernel<false>, a));
+    return counted(cudaLaunchKernelEx(&cfg, kern, a, group, parts));
+}
+
+// Calls f with the kernel's shape for these heads: channels rounded up to 64, 128 or 256; 16 query heads at a time for groups of
+// more than 8 (256 channels: 8, whose sums fill the registers), the rest of a larger group as segments of their own.
+template <class F>
+auto with_shape(bool e4m3, int64_t dim, int64_t group, F&& f) {
+    const bool wide = group > 8;
+    if (e4m3) {
+        if (dim <= 64) return wide ? f(Shape<true, 64, 2, 8, 6>()) : f(Shape<true, 64, 1, 16, 6>());
+        if (dim <= 128) return wide ? f(Shape<true, 128, 2, 8, 6>()) : f(Shape<true, 128, 1, 16, 3>());
+        return f(Shape<true, 256, 1, 8, 3>());
+    }
+    if (dim <= 64) return wide ? f(Shape<false, 64, 2, 8, 6>()) : f(Shape<false, 64, 1, 16, 3>());
+    if (dim <= 128) return wide ? f(Shape<false, 128, 2, 8, 3>()) : f(Shape<false, 128, 1, 8, 3>());
+    return f(Shape<false, 256, 1, 4, 3>());
+}
+
+}  // namespace
+
+size_t paged_attention_scratch(int64_t heads, int64_t kv_heads, int64_t dim, bool e4m3) {
+    return with_shape(e4m3, dim, heads / kv_heads, [](auto s) { return scratch_floats<decltype(s)>(sm_count()) * sizeof(float); });
+}
+
+cudaError_t launch_paged_attention(const AttnArgs& a, cudaStream_t stream) {
+    const int group = a.heads / a.c.kv_heads;
+    return with_shape(a.c.e4m3, a.c.dim, group, [&](auto s) {
+        using S = decltype(s);
+        return launch<S>(a, group, (group + S::kHeads - 1) / S::kHeads, stream);
+    });
 }
 
 }  // namespace fp8lin
