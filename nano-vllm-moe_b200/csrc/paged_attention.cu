@@ -32,6 +32,7 @@ namespace fp8lin {
 namespace {
 
 constexpr int kTile = 16;                       // tokens
+constexpr int kMaxCtas = 192;                   // of a launch: one per SM
 constexpr float kLog2e = 1.4426950408889634f;
 
 template <bool kE4m3_, int kD_, int kN_, int kWarps_, int kStages_>
@@ -118,38 +119,50 @@ __device__ __forceinline__ int tokens_of(const AttnArgs& a, int64_t b, int64_t m
 }
 __device__ __forceinline__ int tiles_of(int len) { return len > kTile ? (int)(((unsigned)len + kTile - 1) / kTile) : 1; }
 
+// (a division of 64 bits is a hundred instructions, on the way of every call)
+__device__ __forceinline__ int64_t quotient(int64_t n, int64_t d) {
+    return ((n | d) >> 32) == 0 ? (int64_t)((uint32_t)n / (uint32_t)d) : n / d;
+}
 // Whose share of `total` tiles among `parts` a tile is in: part p has [total p / parts, total (p + 1) / parts).
-__device__ __forceinline__ int64_t share_begin(int64_t total, int parts, int64_t p) { return total * p / parts; }
-__device__ __forceinline__ int share_of(int64_t total, int parts, int64_t tile) { return (int)(((tile + 1) * parts - 1) / total); }
+__device__ __forceinline__ int64_t share_begin(int64_t total, int parts, int64_t p) { return quotient(total * p, parts); }
+__device__ __forceinline__ int share_of(int64_t total, int parts, int64_t tile) { return (int)quotient((tile + 1) * parts - 1, total); }
 
 struct Piece {                  // part of a segment
     int64_t tile0;              // the segment's first tile in the list, -1: none
     int tiles, b, hc;           // its tiles, sequence, key head and part of its query heads
 };
 
-// Four channels of a query head, the finished sums.
-__device__ __forceinline__ void store4(const AttnArgs& a, int b, int head, int d, float4 v) {
-    if (d >= a.c.dim) return;
-    const int64_t at = (int64_t)b * a.ld_out + (int64_t)head * a.c.dim + d;
-    const uint2 w = {pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w)};
-    if (!a.out_scale) {
-        *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.out) + at) = w;
-        return;
+// Where results go: bf16, or the codes of the bf16 value.
+struct Result {
+    const AttnArgs& a;
+    const ExactDiv div;
+    __device__ __forceinline__ explicit Result(const AttnArgs& args) : a(args), div(args.out_scale ? fmaxf(ld_dep(args.out_scale), 1e-12f) : 1.f) {}
+    // channels d and d + 1 of a query head
+    __device__ __forceinline__ void store2(int b, int head, int d, uint32_t w) const {
+        const int64_t at = (int64_t)b * a.ld_out + (int64_t)head * a.c.dim + d;
+        if (a.out_scale) *reinterpret_cast<uint16_t*>(static_cast<unsigned char*>(a.out) + at) = cvt_e4m3x2(div(bf16_lo(w)), div(bf16_hi(w)));
+        else *reinterpret_cast<uint32_t*>(static_cast<__nv_bfloat16*>(a.out) + at) = w;
     }
-    const ExactDiv div(fmaxf(ld_dep(a.out_scale), 1e-12f));
-    const uint32_t lo = cvt_e4m3x2(div(bf16_lo(w.x)), div(bf16_hi(w.x))), hi = cvt_e4m3x2(div(bf16_lo(w.y)), div(bf16_hi(w.y)));
-    *reinterpret_cast<uint32_t*>(static_cast<unsigned char*>(a.out) + at) = lo | (hi << 16);
-}
-// ... and two, from the fragments of a warp that had the whole segment
-__device__ __forceinline__ void store2(const AttnArgs& a, int b, int head, int d, uint32_t w) {
-    const int64_t at = (int64_t)b * a.ld_out + (int64_t)head * a.c.dim + d;
-    if (!a.out_scale) {
-        *reinterpret_cast<uint32_t*>(static_cast<__nv_bfloat16*>(a.out) + at) = w;
-        return;
+    // A fragment of the sums O^T of 16 channels from c * 16 on and of query heads n * 8 + 2 t4 (x, z) and n * 8 + 2 t4 + 1 (y, w),
+    // times those heads' `inv`.  All lanes of a warp together.
+    template <bool kE4m3>
+    __device__ __forceinline__ void store(int b, int head0, int heads, int c, int n, float4 v, float2 inv) const {
+        const int g = (threadIdx.x & 31) >> 2, t4 = threadIdx.x & 3;
+        if (c * 16 >= a.c.dim) return;
+        if (kE4m3) {                                                              // rows g and g + 8: channels 2g and 2g + 1
+            const int col = n * 8 + 2 * t4;
+            if (col < heads) store2(b, head0 + col, c * 16 + 2 * g, pack_bf16x2(v.x * inv.x, v.z * inv.x));
+            if (col + 1 < heads) store2(b, head0 + col + 1, c * 16 + 2 * g, pack_bf16x2(v.y * inv.y, v.w * inv.y));
+        } else {                                                                  // channels g and g + 8: transposed, a lane has two of head g
+            const uint32_t lo = transposed(pack_bf16x2(v.x * inv.x, v.y * inv.y)), hi = transposed(pack_bf16x2(v.z * inv.x, v.w * inv.y));
+            const int col = n * 8 + g;
+            if (col < heads) {
+                store2(b, head0 + col, c * 16 + 2 * t4, lo);
+                store2(b, head0 + col, c * 16 + 8 + 2 * t4, hi);
+            }
+        }
     }
-    const ExactDiv div(fmaxf(ld_dep(a.out_scale), 1e-12f));
-    *reinterpret_cast<uint16_t*>(static_cast<unsigned char*>(a.out) + at) = cvt_e4m3x2(div(bf16_lo(w)), div(bf16_hi(w)));
-}
+};
 
 // Scratch: the sums of a warp's first piece where it went on to another segment, then two pieces per CTA with their statistics.
 template <class S>
@@ -163,12 +176,11 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
     constexpr bool kE4m3 = S::kE4m3;
     constexpr int kD = S::kD, kN = S::kN, kHeads = S::kHeads, kWarps = S::kWarps, kStages = S::kStages, kRow = S::kRow, kPiece = S::kPiece;
     extern __shared__ __align__(1024) unsigned char ring[];
-    __shared__ int64_t s_scan[kWarps], s_base[kWarps];
-    __shared__ int s_b[kWarps];
     __shared__ Piece s_piece[2 * kWarps];
-    __shared__ float s_m[2 * kWarps][kHeads], s_l[2 * kWarps][kHeads];
-    __shared__ uint32_t s_run[2 * kWarps];      // the pieces of a run (bits), pieces of one segment
-    __shared__ int s_runs, s_open[2], s_last[2];
+    // (read two heads at a time)
+    __shared__ __align__(16) float s_m[2 * kWarps][kHeads], s_l[2 * kWarps][kHeads], s_f[2 * kWarps][kHeads], s_inv[kHeads], s_share[kMaxCtas][kHeads];
+    __shared__ int s_entry[2 * kWarps], s_first[2 * kWarps + 1];                 // the pieces that there are, and where a run of one segment's begins
+    __shared__ int s_open[2], s_last[2];
 
     pdl_launch_dependents();
     pdl_wait();
@@ -176,71 +188,33 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
     const int segments = a.c.kv_heads * parts;                                   // per sequence
     const int64_t most64 = a.max_pages * a.c.block_size, most = most64 < 0x7fffffff ? most64 : 0x7fffffff;
 
-    // ---- shares -----------------------------------------------------------------------------------------------------
-    auto block_scan = [&](int64_t v, int64_t& before, int64_t& all) {             // exclusive sum over the threads, and all of it
-        int64_t x = v;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
-            if (lane >= o) x += y;
+    // ---- shares: every warp for itself, a lane for a stretch of sequences -------------------------------------------
+    const int stretch = (a.batch + 31) >> 5, lane_b = lane * stretch;
+    int64_t mine = 0;
+#pragma unroll 4
+    for (int i = 0; i < stretch; ++i) {
+        if (lane_b + i < a.batch) {
+            const int len = ld_dep(a.lens + lane_b + i);
+            if (len > most && blockIdx.x == 0) report_status(a.status, kDevBadPage);
+            mine += tiles_of(len < most ? len : (int)most);
         }
-        if (lane == 31) s_scan[warp] = x;
-        __syncthreads();
-        before = x - v;
-        all = 0;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-            if (w < warp) before += s_scan[w];
-            all += s_scan[w];
-        }
-        __syncthreads();
-    };
-    if (tid < 2) s_open[tid] = -1;
-    const bool once = a.batch <= S::kThreads;
-    int64_t total = 0, before = 0;
-    int my_tiles = 0;
-    auto look = [&](int b) {
-        if (b >= a.batch) return 0;
-        if (blockIdx.x == 0 && (int64_t)ld_dep(a.lens + b) > most) report_status(a.status, kDevBadPage);
-        return tiles_of(tokens_of(a, b, most));
-    };
-    if (once) {
-        my_tiles = look(tid);
-        block_scan((int64_t)my_tiles * segments, before, total);
-    } else {
-        int64_t sum = 0, unused;
-        for (int b = tid; b < a.batch; b += S::kThreads) sum += (int64_t)look(b) * segments;
-        block_scan(sum, unused, total);
     }
+    mine *= segments;
+    int64_t before = mine;                                                        // inclusive sum
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int64_t y = __shfl_up_sync(0xffffffffu, before, o);
+        if (lane >= o) before += y;
+    }
+    const int64_t total = __shfl_sync(0xffffffffu, before, 31);
+    before -= mine;
     // one tile per warp at least
     const int64_t wanted = (total + kWarps - 1) / kWarps;
     const int ctas = wanted < gridDim.x ? (int)wanted : (int)gridDim.x;
     if ((int)blockIdx.x >= ctas) return;
     const int64_t cta0 = share_begin(total, ctas, blockIdx.x), cta1 = share_begin(total, ctas, blockIdx.x + 1);
-    auto place = [&](int b, int tiles, int64_t at) {                               // which warps begin in sequence b's tiles
-        const int64_t end = at + (int64_t)tiles * segments;
-        if (tiles == 0 || end <= cta0 || at >= cta1) return;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-            const int64_t begin = cta0 + share_begin(cta1 - cta0, kWarps, w);
-            if (begin >= at && begin < end) { s_b[w] = b; s_base[w] = at; }
-        }
-    };
-    if (once) {
-        place(tid, my_tiles, before);
-    } else {
-        int64_t base = 0;
-        for (int b0 = 0; b0 < a.batch && base < cta1; b0 += S::kThreads) {
-            const int b = b0 + tid, tiles = b < a.batch ? tiles_of(tokens_of(a, b, most)) : 0;
-            int64_t all;
-            block_scan((int64_t)tiles * segments, before, all);
-            place(b, tiles, base + before);
-            base += all;
-        }
-    }
-    __syncthreads();
-    const int64_t begin = cta0 + share_begin(cta1 - cta0, kWarps, warp);
-    const int64_t todo = cta0 + share_begin(cta1 - cta0, kWarps, warp + 1) - begin;
+    const int64_t begin = cta0 + (cta1 - cta0) * warp / kWarps, todo = cta0 + (cta1 - cta0) * (warp + 1) / kWarps - begin;
+    if (tid < 2) s_open[tid] = -1;
 
     // ---- a warp's tiles -----------------------------------------------------------------------------------------------
     unsigned char* const my_ring = ring + warp * (kStages * S::kStageBytes);
@@ -254,12 +228,18 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
         if (paged16 && in.t * kTile < in.len) page = ld_dep(a.tables + (int64_t)in.b * a.ld_tables + page_at);
     };
     if (todo > 0) {
-        const int b = s_b[warp];
-        const int64_t inside = begin - s_base[warp];
+        const int where = __ffs(__ballot_sync(0xffffffffu, begin >= before && begin < before + mine)) - 1;
+        int64_t inside = begin - __shfl_sync(0xffffffffu, before, where);
+        int b = where * stretch;
+        for (;; ++b) {
+            in.len = tokens_of(a, b, most);
+            in.tiles = tiles_of(in.len);
+            const int64_t all = (int64_t)in.tiles * segments;
+            if (inside < all) break;                                              // (it is one of the stretch's)
+            inside -= all;
+        }
         in.b = b;
-        in.len = tokens_of(a, b, most);
-        in.tiles = tiles_of(in.len);
-        in.hc = (int)(inside / in.tiles);
+        in.hc = (int)quotient(inside, in.tiles);
         in.t = (int)(inside - (int64_t)in.hc * in.tiles);
         at = in;
         page_at = in.t * kTile / a.c.block_size;
@@ -344,6 +324,7 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
         }
     };
 
+    const Result result(a);
     uint32_t q[kD / 16][kN][2];
     float o[kD / 16][kN][4], m[kN][2], l[kN][2], to_score[kN][2];
     int value_exp = 15;                                                            // exponent field that the values' scales are relative to
@@ -378,16 +359,18 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
                 top = max(top & 0xffffu, top >> 16);
                 top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
                 top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                const int e = (int)(top >> 7), up = e == 255 ? 0 : 14 + 127 - (e == 0 ? 1 : e);
+                const int e = (int)(top >> 7), up = e == 255 ? 0 : 14 + 127 - (e == 0 ? 1 : e);       // -113 .. 140: as two factors
+                const float up1 = __int_as_float((127 + (up >> 1)) << 23), up2 = __int_as_float((127 + up - (up >> 1)) << 23);
+                const float down1 = __int_as_float((127 - (up >> 1)) << 23), down2 = __int_as_float((127 - up + (up >> 1)) << 23);
 #pragma unroll
                 for (int s = 0; s < kD / 16; ++s)
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
                         const uint32_t w = q[s][n][i];
-                        q[s][n][i] = pack_f16x2(ldexpf(bf16_lo(w), up), ldexpf(bf16_hi(w), up));
+                        q[s][n][i] = pack_f16x2(bf16_lo(w) * up1 * up2, bf16_hi(w) * up1 * up2);
                     }
 #pragma unroll
-                for (int i = 0; i < 2; ++i) to_score[n][i] = ldexpf(base, -__shfl_sync(0xffffffffu, up, (2 * t4 + i) * 4));
+                for (int i = 0; i < 2; ++i) to_score[n][i] = base * __shfl_sync(0xffffffffu, down1, (2 * t4 + i) * 4) * __shfl_sync(0xffffffffu, down2, (2 * t4 + i) * 4);
             } else {
                 to_score[n][0] = to_score[n][1] = base;
             }
@@ -525,23 +508,18 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
             }
         }
     };
-    // the channels of o[c][.][0..1] and o[c][.][2..3]
-    auto channel = [&](int c, int half) { return kE4m3 ? c * 16 + 2 * g + half : c * 16 + g + 8 * half; };
-    // A piece's sums with their statistics; `last`: the warp's last piece, kept in shared memory, else in scratch.
+    // A piece's sums, as they lie in the lanes, with their statistics; `last`: the warp's last piece, kept in shared memory, else in scratch.
     auto keep_piece = [&](bool last, float* sums) {
         const int e = 2 * warp + last;
 #pragma unroll
-        for (int n = 0; n < kN; ++n)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int col = n * 8 + 2 * t4 + i;
-                if (g == 0) { s_m[e][col] = m[n][i]; s_l[e][col] = l[n][i]; }
-#pragma unroll
-                for (int c = 0; c < kD / 16; ++c) {
-                    sums[col * kD + channel(c, 0)] = o[c][n][i];
-                    sums[col * kD + channel(c, 1)] = o[c][n][2 + i];
-                }
+        for (int n = 0; n < kN; ++n) {
+            if (g == 0) {
+                *reinterpret_cast<float2*>(&s_m[e][n * 8 + 2 * t4]) = {m[n][0], m[n][1]};
+                *reinterpret_cast<float2*>(&s_l[e][n * 8 + 2 * t4]) = {l[n][0], l[n][1]};
             }
+#pragma unroll
+            for (int c = 0; c < kD / 16; ++c) reinterpret_cast<float4*>(sums)[(c * kN + n) * 32 + lane] = {o[c][n][0], o[c][n][1], o[c][n][2], o[c][n][3]};
+        }
     };
     float* const early = a.partial + ((int64_t)blockIdx.x * kWarps + warp) * kPiece;
     bool kept = false;
@@ -560,8 +538,10 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
             if (ahead + 1 < todo) next_page();
         }
         copies_end();
-        if (i < 0) continue;
-        if (i == 0 || at.t == 0) begin_segment();
+        if (i < 0) {
+            if (i == -1 && todo > 0) begin_segment();
+            continue;
+        }
         work_on(from);
         from = from + 1 == kStages ? 0 : from + 1;
         const bool ends = at.t + 1 == at.tiles, last = i + 1 == todo;
@@ -579,30 +559,14 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
                         for (int c = 0; c < kD / 16; ++c) { o[c][n][j] *= back; o[c][n][2 + j] *= back; }
                 }
             if (ends && i >= at.t) {                                               // the whole segment was this warp's
-                const int part = at.hc % parts, head0 = at.hc / parts * group + part * kHeads, heads = min(kHeads, group - part * kHeads);
+                const int part = at.hc % parts;
 #pragma unroll
                 for (int n = 0; n < kN; ++n) {
-                    float inv[2];
+                    const float2 inv = at.len > 0 ? float2{__fdiv_rn(1.f, l[n][0]), __fdiv_rn(1.f, l[n][1])} : float2{0.f, 0.f};
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) inv[j] = at.len > 0 ? __fdiv_rn(1.f, l[n][j]) : 0.f;
-#pragma unroll
-                    for (int c = 0; c < kD / 16; ++c) {
-                        if (c * 16 >= a.c.dim) continue;
-                        if (kE4m3) {
-#pragma unroll
-                            for (int j = 0; j < 2; ++j) {
-                                const int col = n * 8 + 2 * t4 + j;
-                                if (col < heads) store2(a, at.b, head0 + col, channel(c, 0), pack_bf16x2(o[c][n][j] * inv[j], o[c][n][2 + j] * inv[j]));
-                            }
-                        } else {
-                            const int col = n * 8 + g;
-#pragma unroll
-                            for (int h = 0; h < 2; ++h) {                          // lanes of a head side by side: its channels 2 t4, 2 t4 + 1
-                                const uint32_t w = transposed(pack_bf16x2(o[c][n][2 * h] * inv[0], o[c][n][2 * h + 1] * inv[1]));
-                                if (col < heads) store2(a, at.b, head0 + col, c * 16 + 8 * h + 2 * t4, w);
-                            }
-                        }
-                    }
+                    for (int c = 0; c < kD / 16; ++c)
+                        result.store<kE4m3>(at.b, at.hc / parts * group + part * kHeads, min(kHeads, group - part * kHeads), c, n,
+                                            {o[c][n][0], o[c][n][1], o[c][n][2], o[c][n][3]}, inv);
                 }
             } else {
                 if (lane == 0) s_piece[2 * warp + last] = {begin + i - at.t, at.tiles, at.b, at.hc};
@@ -620,70 +584,98 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
                     at.tiles = tiles_of(at.len);
                 }
             }
+            if (i + 1 < todo) begin_segment();
         }
     }
 
     // ---- pieces of a segment in this CTA ------------------------------------------------------------------------------
     copies_wait<0>();
     __syncthreads();
-    float* const sums = reinterpret_cast<float*>(ring);                            // [warp][head][channel], over the rings
+    float* const sums = reinterpret_cast<float*>(ring);                            // [warp][piece], over the rings
     if (kept) keep_piece(true, sums + warp * kPiece);
-    if (warp == 0) {
-        const int64_t seg = lane < 2 * kWarps ? s_piece[lane].tile0 : -1;
-        const uint32_t there = __ballot_sync(0xffffffffu, seg >= 0);
-        const uint32_t below = there & ((1u << lane) - 1);
-        const int64_t prev = __shfl_sync(0xffffffffu, seg, below ? 31 - __clz(below) : lane);
-        const bool first = seg >= 0 && (below == 0 || prev != seg);
-        const uint32_t firsts = __ballot_sync(0xffffffffu, first);
-        if (first) {
-            const uint32_t above = firsts & ~((2u << lane) - 1);
-            const int run = __popc(firsts & ((1u << lane) - 1));
-            s_run[run] = there & ~((1u << lane) - 1) & (above ? (1u << (__ffs(above) - 1)) - 1 : 0xffffffffu);
+    __syncthreads();
+    // A lane for a piece (two per warp, the second its last), every warp for itself: runs of pieces of one segment.
+    const int64_t seg = lane < 2 * kWarps ? s_piece[lane].tile0 : -1;
+    const uint32_t there = __ballot_sync(0xffffffffu, seg >= 0), below = there & ((1u << lane) - 1);
+    const int64_t prev = __shfl_sync(0xffffffffu, seg, below ? 31 - __clz(below) : lane);
+    const uint32_t firsts = __ballot_sync(0xffffffffu, seg >= 0 && (below == 0 || prev != seg));
+    if (firsts == 0) return;
+    const int runs = __popc(firsts);
+    const uint32_t upto = firsts & ((2u << lane) - 1), beyond = firsts & ~((2u << lane) - 1);
+    const int first = upto ? 31 - __clz(upto) : 0, end = beyond ? __ffs(beyond) - 1 : 32;      // lanes of this lane's run
+    if (warp == 0 && seg >= 0) {
+        s_entry[__popc(below)] = lane;
+        if (lane == first) {
             const Piece p = s_piece[lane];
+            const int run = __popc(upto) - 1;
+            s_first[run] = __popc(below);
+            if (run == runs - 1) s_first[runs] = __popc(there);
             if (p.tile0 < cta0) s_open[0] = run;
             else if (p.tile0 + p.tiles > cta1) s_open[1] = run;
         }
-        if (lane == 0) s_runs = __popc(firsts);
+    }
+    // the weights of a run's pieces, a warp for a query head
+    for (int col = warp; col < kHeads; col += kWarps) {
+        const float pm = seg >= 0 ? s_m[lane][col] : -INFINITY;
+        float top = pm, sum;
+#pragma unroll
+        for (int x = 1; x < 32; x <<= 1) {
+            const float y = __shfl_up_sync(0xffffffffu, top, x);
+            if (lane - x >= first) top = fmaxf(top, y);
+        }
+        top = __shfl_sync(0xffffffffu, top, end - 1);
+        const float f = weight_of(pm, top);
+        sum = seg >= 0 ? f * s_l[lane][col] : 0.f;
+#pragma unroll
+        for (int x = 1; x < 32; x <<= 1) {
+            const float y = __shfl_up_sync(0xffffffffu, sum, x);
+            if (lane - x >= first) sum += y;
+        }
+        sum = __shfl_sync(0xffffffffu, sum, end - 1);
+        if (seg >= 0) {
+            s_f[lane][col] = f;
+            if (lane == first) { s_m[lane][col] = top; s_l[lane][col] = sum; }     // (this lane's alone from here on)
+        }
     }
     __syncthreads();
-    constexpr int kUnits = kPiece / 4;                                             // four channels of one head
-    float* const pieces = a.partial + (int64_t)gridDim.x * kWarps * kPiece;         // [CTA][2][sums | m | l]
+    constexpr int kUnits = kPiece / 4;                                             // fragments of a lane: two heads, two channels
     constexpr int kOut = kPiece + 2 * kHeads;
-    const int runs = s_runs;
+    float* const pieces = a.partial + (int64_t)gridDim.x * kWarps * kPiece;         // [CTA][2][sums | m | l]
     for (int x = tid; x < runs * kUnits; x += S::kThreads) {
-        const int run = x / kUnits, unit = x - run * kUnits, col = unit / (kD / 4), d = unit % (kD / 4) * 4;
-        const uint32_t members = s_run[run];
-        const Piece p = s_piece[__ffs(members) - 1];
-        float top = -INFINITY, total_l = 0.f;
-        for (uint32_t left = members; left; left &= left - 1) top = fmaxf(top, s_m[__ffs(left) - 1][col]);
+        const int run = x / kUnits, unit = x % kUnits, col = (unit >> 5) % kN * 8 + 2 * t4;
+        const int e0 = s_entry[s_first[run]];
         float4 v = {0.f, 0.f, 0.f, 0.f};
-        for (uint32_t left = members; left; left &= left - 1) {
-            const int e = __ffs(left) - 1;
-            const float f = weight_of(s_m[e][col], top);
+#pragma unroll 4
+        for (int k = s_first[run]; k < s_first[run + 1]; ++k) {
+            const int e = s_entry[k];
+            const float2 f = *reinterpret_cast<const float2*>(&s_f[e][col]);
             const float* from = (e & 1) ? sums + (e >> 1) * kPiece : a.partial + ((int64_t)blockIdx.x * kWarps + (e >> 1)) * kPiece;
-            const float4 w = *reinterpret_cast<const float4*>(from + col * kD + d);
-            total_l += f * s_l[e][col];
-            v.x += f * w.x; v.y += f * w.y; v.z += f * w.z; v.w += f * w.w;
+            const float4 w = reinterpret_cast<const float4*>(from)[unit];
+            v.x += f.x * w.x; v.y += f.y * w.y; v.z += f.x * w.z; v.w += f.y * w.w;
         }
-        const int part = p.hc % parts, head = p.hc / parts * group + part * kHeads + col;
+        const float2 sum = *reinterpret_cast<const float2*>(&s_l[e0][col]);
         if (run == s_open[0] || run == s_open[1]) {
             float* out = pieces + ((int64_t)blockIdx.x * 2 + (run == s_open[1])) * kOut;
-            *reinterpret_cast<float4*>(out + col * kD + d) = v;
-            if (d == 0) { out[kPiece + col] = top; out[kPiece + kHeads + col] = total_l; }
-        } else if (part * kHeads + col < group) {
-            const float inv = __fdiv_rn(1.f, total_l);
-            store4(a, p.b, head, d, {v.x * inv, v.y * inv, v.z * inv, v.w * inv});
+            reinterpret_cast<float4*>(out)[unit] = v;
+            if (unit >> 5 < kN && g == 0) {                                        // (the first channels' fragments have every head once)
+                *reinterpret_cast<float2*>(out + kPiece + col) = *reinterpret_cast<const float2*>(&s_m[e0][col]);
+                *reinterpret_cast<float2*>(out + kPiece + kHeads + col) = sum;
+            }
+        } else {
+            const Piece p = s_piece[e0];
+            const int part = p.hc % parts;
+            result.store<kE4m3>(p.b, p.hc / parts * group + part * kHeads, min(kHeads, group - part * kHeads), (unit >> 5) / kN, (unit >> 5) % kN, v,
+                                {__fdiv_rn(1.f, sum.x), __fdiv_rn(1.f, sum.y)});
         }
     }
 
     // ---- segments that other CTAs have pieces of: the last one to come joins them --------------------------------------
     if (s_open[0] < 0 && s_open[1] < 0) return;
-    __threadfence();
     __syncthreads();
     if (tid < 2) {
         bool last = false;
         if (s_open[tid] >= 0) {
-            const Piece p = s_piece[__ffs(s_run[s_open[tid]]) - 1];
+            const Piece p = s_piece[s_entry[s_first[s_open[tid]]]];
             const int c0 = share_of(total, ctas, p.tile0), c1 = share_of(total, ctas, p.tile0 + p.tiles - 1);
             __threadfence();
             last = atomicAdd(a.counters + c0, 1) == c1 - c0;
@@ -696,50 +688,63 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
 #pragma unroll 1
     for (int w = 0; w < 2; ++w) {
         if (!s_last[w]) continue;
-        const Piece p = s_piece[__ffs(s_run[s_open[w]]) - 1];
-        const int c0 = share_of(total, ctas, p.tile0), c1 = share_of(total, ctas, p.tile0 + p.tiles - 1);
-        const int part = p.hc % parts, head0 = p.hc / parts * group + part * kHeads;
-        for (int unit = tid; unit < kUnits; unit += S::kThreads) {
-            const int col = unit / (kD / 4), d = unit % (kD / 4) * 4;
-            float top = -INFINITY, total_l = 0.f;
-            float4 v = {0.f, 0.f, 0.f, 0.f};
-            constexpr int kAtOnce = 8;
-            for (int c = c0; c <= c1; c += kAtOnce) {
-                float4 x[kAtOnce];
-                float xm[kAtOnce], xl[kAtOnce], now = top;
+        const Piece p = s_piece[s_entry[s_first[s_open[w]]]];
+        const int c0 = share_of(total, ctas, p.tile0), count = share_of(total, ctas, p.tile0 + p.tiles - 1) - c0 + 1;
+        auto piece_of = [&](int i) { return pieces + ((int64_t)(c0 + i) * 2 + (i == 0)) * kOut; };
+        for (int col = warp; col < kHeads; col += kWarps) {                        // a warp for a query head, a lane for a few CTAs
+            float pm[kMaxCtas / 32], pl[kMaxCtas / 32], top = -INFINITY, sum = 0.f;
 #pragma unroll
-                for (int j = 0; j < kAtOnce; ++j) {
-                    xm[j] = -INFINITY;
-                    xl[j] = 0.f;
-                    x[j] = {0.f, 0.f, 0.f, 0.f};
-                    if (c + j <= c1) {
-                        const float* from = pieces + ((int64_t)(c + j) * 2 + (c + j == c0)) * kOut;
-                        const uint4 raw = ld_dep_l2(reinterpret_cast<const uint4*>(from + col * kD + d));
-                        x[j] = {__uint_as_float(raw.x), __uint_as_float(raw.y), __uint_as_float(raw.z), __uint_as_float(raw.w)};
-                        xm[j] = ld_dep_l2(from + kPiece + col);
-                        xl[j] = ld_dep_l2(from + kPiece + kHeads + col);
-                    }
+            for (int i = 0; i < kMaxCtas / 32; ++i) {
+                pm[i] = -INFINITY;
+                pl[i] = 0.f;
+                if (i * 32 + lane < count) {
+                    pm[i] = ld_dep_l2(piece_of(i * 32 + lane) + kPiece + col);
+                    pl[i] = ld_dep_l2(piece_of(i * 32 + lane) + kPiece + kHeads + col);
                 }
-#pragma unroll
-                for (int j = 0; j < kAtOnce; ++j) now = fmaxf(now, xm[j]);
-                const float f0 = weight_of(top, now);
-                total_l *= f0;
-                v.x *= f0; v.y *= f0; v.z *= f0; v.w *= f0;
-#pragma unroll
-                for (int j = 0; j < kAtOnce; ++j) {
-                    const float f = weight_of(xm[j], now);
-                    total_l += f * xl[j];
-                    v.x += f * x[j].x; v.y += f * x[j].y; v.z += f * x[j].z; v.w += f * x[j].w;
-                }
-                top = now;
+                top = fmaxf(top, pm[i]);
             }
-            if (part * kHeads + col < group) {
-                const float inv = __fdiv_rn(1.f, total_l);
-                store4(a, p.b, head0 + col, d, {v.x * inv, v.y * inv, v.z * inv, v.w * inv});
+            for (int x = 16; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+#pragma unroll
+            for (int i = 0; i < kMaxCtas / 32; ++i) {
+                const float f = weight_of(pm[i], top);
+                sum += f * pl[i];
+                if (i * 32 + lane < count) s_share[i * 32 + lane][col] = f;
             }
+            for (int x = 16; x; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+            if (lane == 0) s_inv[col] = __fdiv_rn(1.f, sum);
         }
+        __syncthreads();
+        // kSlices threads share a fragment's pieces
+        constexpr int kSlices = S::kThreads > kUnits ? S::kThreads / kUnits : 1;
+        for (int x = tid; x < kSlices * kUnits; x += S::kThreads) {
+            const int unit = x % kUnits, slice = x / kUnits, n = (unit >> 5) % kN, col = n * 8 + 2 * t4;
+            float4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+            for (int i = slice; i < count; i += kSlices) {
+                const uint4 raw = ld_dep_l2(reinterpret_cast<const uint4*>(piece_of(i)) + unit);
+                const float2 f = *reinterpret_cast<const float2*>(&s_share[i][col]);
+                v.x += f.x * __uint_as_float(raw.x); v.y += f.y * __uint_as_float(raw.y);
+                v.z += f.x * __uint_as_float(raw.z); v.w += f.y * __uint_as_float(raw.w);
+            }
+            if (kSlices > 1) {
+                if (slice > 0) reinterpret_cast<float4*>(sums)[(slice - 1) * kUnits + unit] = v;
+                __syncthreads();                                                   // (one turn for every thread)
+                if (slice > 0) continue;
+#pragma unroll
+                for (int k = 1; k < kSlices; ++k) {
+                    const float4 y = reinterpret_cast<const float4*>(sums)[(k - 1) * kUnits + unit];
+                    v.x += y.x; v.y += y.y; v.z += y.z; v.w += y.w;
+                }
+            }
+            const int part = p.hc % parts;
+            result.store<kE4m3>(p.b, p.hc / parts * group + part * kHeads, min(kHeads, group - part * kHeads), (unit >> 5) / kN, n, v,
+                                *reinterpret_cast<const float2*>(&s_inv[col]));
+        }
+        __syncthreads();                                                           // s_share, s_inv and the sums are free again
     }
 }
+
+int attention_ctas() { return sm_count() < kMaxCtas ? sm_count() : kMaxCtas; }
 
 template <class S>
 cudaError_t launch(const AttnArgs& a, int group, int parts, cudaStream_t stream) {
@@ -754,7 +759,7 @@ cudaError_t launch(const AttnArgs& a, int group, int parts, cudaStream_t stream)
         if (dev < 64) ready.fetch_or(1ull << dev, std::memory_order_release);
     }
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)sm_count());
+    cfg.gridDim = dim3((unsigned)attention_ctas());
     cfg.blockDim = dim3(S::kThreads);
     cfg.dynamicSmemBytes = S::kSmem;
     cfg.stream = stream;
@@ -782,7 +787,7 @@ auto with_shape(bool e4m3, int64_t dim, int64_t group, F&& f) {
 }  // namespace
 
 size_t paged_attention_scratch(int64_t heads, int64_t kv_heads, int64_t dim, bool e4m3) {
-    return with_shape(e4m3, dim, heads / kv_heads, [](auto s) { return scratch_floats<decltype(s)>(sm_count()) * sizeof(float); });
+    return with_shape(e4m3, dim, heads / kv_heads, [](auto s) { return scratch_floats<decltype(s)>(attention_ctas()) * sizeof(float); });
 }
 
 cudaError_t launch_paged_attention(const AttnArgs& a, cudaStream_t stream) {
