@@ -59,6 +59,9 @@ __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there) {
     asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
 }
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
 __device__ __forceinline__ void copy4(uint32_t dst, const void* src, bool there) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(there ? 4 : 0) : "memory");
 }
@@ -91,8 +94,11 @@ __device__ __forceinline__ float exp2_approx(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
-// exp2(m - top) for a maximum that may be that of nothing
-__device__ __forceinline__ float weight_of(float m, float top) { return m == -INFINITY ? 0.f : exp2_approx(m - top); }
+// The reference of no score at all; exp2(kNone - m) is 0 for that of any.
+constexpr float kNone = -3.402823466e38f;
+// Weights are relative to a score that is at most 2^kSlack below the largest: it follows the maximum only where that
+// runs away from it, so that the sums are rescaled once or twice per segment and not with every new maximum.
+constexpr float kSlack = 8.f;
 __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&h);
@@ -110,6 +116,13 @@ __device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t&
         hi = pack_bf16x2(x, y);
         lo = pack_bf16x2(x - bf16_lo(hi), y - bf16_hi(hi));
     }
+}
+
+// Adds one: what this block wrote before is there for whoever sees the sum, and what others wrote before theirs for this block.
+__device__ __forceinline__ int arrive(int* counter) {
+    int old;
+    asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(old) : "l"(counter) : "memory");
+    return old;
 }
 
 // Tiles of a sequence; an empty one has one as well, of nothing, so that its zeros are written like any result.
@@ -180,7 +193,7 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
     // (read two heads at a time)
     __shared__ __align__(16) float s_m[2 * kWarps][kHeads], s_l[2 * kWarps][kHeads], s_f[2 * kWarps][kHeads], s_inv[kHeads], s_share[kMaxCtas][kHeads];
     __shared__ int s_entry[2 * kWarps], s_first[2 * kWarps + 1];                 // the pieces that there are, and where a run of one segment's begins
-    __shared__ int s_open[2], s_last[2];
+    __shared__ int s_open[2], s_last[2], s_cta0[2], s_ctas[2];                   // runs that other CTAs have pieces of; which CTAs
 
     pdl_launch_dependents();
     pdl_wait();
@@ -191,7 +204,7 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
     // ---- shares: every warp for itself, a lane for a stretch of sequences -------------------------------------------
     const int stretch = (a.batch + 31) >> 5, lane_b = lane * stretch;
     int64_t mine = 0;
-#pragma unroll 4
+#pragma unroll 8
     for (int i = 0; i < stretch; ++i) {
         if (lane_b + i < a.batch) {
             const int len = ld_dep(a.lens + lane_b + i);
@@ -213,115 +226,153 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
     const int ctas = wanted < gridDim.x ? (int)wanted : (int)gridDim.x;
     if ((int)blockIdx.x >= ctas) return;
     const int64_t cta0 = share_begin(total, ctas, blockIdx.x), cta1 = share_begin(total, ctas, blockIdx.x + 1);
-    const int64_t begin = cta0 + (cta1 - cta0) * warp / kWarps, todo = cta0 + (cta1 - cta0) * (warp + 1) / kWarps - begin;
+    const int64_t begin = cta0 + (cta1 - cta0) * warp / kWarps, todo64 = cta0 + (cta1 - cta0) * (warp + 1) / kWarps - begin;
+    const int todo = (int)(todo64 < 0x7fffffff ? todo64 : 0x7fffffff);
     if (tid < 2) s_open[tid] = -1;
 
     // ---- a warp's tiles -----------------------------------------------------------------------------------------------
     unsigned char* const my_ring = ring + warp * (kStages * S::kStageBytes);
+    const uint32_t my_ring_at = smem_addr(my_ring);
     const int row_bytes = a.c.dim * (kE4m3 ? 1 : 2);
     const bool paged16 = a.c.block_size % kTile == 0;
     const int g = lane >> 2, t4 = lane & 3;
+    if (row_bytes < kRow) {                                         // channels behind head_dim: zeros once, they are never copied to
+        for (int i = lane * 16; i < kStages * S::kStageBytes; i += 512) *reinterpret_cast<uint4*>(my_ring + i) = {0, 0, 0, 0};
+        __syncwarp();
+    }
 
     struct Place { int b, hc, t, len, tiles; } in, at;              // of the next tile to copy, and to work on
-    int next_len = 0, page = 0, page_at = 0, page_off = 0;
-    auto next_page = [&] {                                          // of tile `in`, asked for one tile early
-        if (paged16 && in.t * kTile < in.len) page = ld_dep(a.tables + (int64_t)in.b * a.ld_tables + page_at);
+    // Pages of `in` where they hold whole tiles: 32 entries of its table at a time, a lane each, from page_base on
+    int next_len = 0, pages = 0, next_pages = 0, page_base = 0, page_at = 0, page_off = 0;
+    auto table_entry = [&](int b, int len, int i) {
+        return (int64_t)i * a.c.block_size < len ? ld_dep(a.tables + (int64_t)b * a.ld_tables + i) : 0;
+    };
+    auto look_ahead = [&] {
+        if (in.b + 1 < a.batch) {
+            next_len = tokens_of(a, in.b + 1, most);
+            if (paged16) next_pages = table_entry(in.b + 1, next_len, lane);
+        }
     };
     if (todo > 0) {
-        const int where = __ffs(__ballot_sync(0xffffffffu, begin >= before && begin < before + mine)) - 1;
-        int64_t inside = begin - __shfl_sync(0xffffffffu, before, where);
-        int b = where * stretch;
-        for (;; ++b) {
-            in.len = tokens_of(a, b, most);
-            in.tiles = tiles_of(in.len);
-            const int64_t all = (int64_t)in.tiles * segments;
-            if (inside < all) break;                                              // (it is one of the stretch's)
-            inside -= all;
+        int64_t inside = begin - before;
+        const int where = __ffs(__ballot_sync(0xffffffffu, inside >= 0 && inside < mine)) - 1;
+        inside = __shfl_sync(0xffffffffu, inside, where);
+        for (int b0 = where * stretch;; b0 += 32) {                               // (it is one of the stretch's)
+            const int len = b0 + lane < a.batch ? tokens_of(a, b0 + lane, most) : 0;
+            const int64_t all = b0 + lane < a.batch ? (int64_t)tiles_of(len) * segments : 0;
+            int64_t upto = all;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int64_t y = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += y;
+            }
+            const uint32_t beyond = __ballot_sync(0xffffffffu, upto > inside);
+            if (beyond) {
+                const int w = __ffs(beyond) - 1;
+                in.b = b0 + w;
+                in.len = __shfl_sync(0xffffffffu, len, w);
+                inside -= __shfl_sync(0xffffffffu, upto - all, w);
+                break;
+            }
+            inside -= __shfl_sync(0xffffffffu, upto, 31);
         }
-        in.b = b;
+        in.tiles = tiles_of(in.len);
         in.hc = (int)quotient(inside, in.tiles);
         in.t = (int)(inside - (int64_t)in.hc * in.tiles);
         at = in;
-        page_at = in.t * kTile / a.c.block_size;
-        page_off = in.t * kTile - page_at * a.c.block_size;
-        next_page();
-        if (b + 1 < a.batch) next_len = tokens_of(a, b + 1, most);
+        if (paged16) {
+            page_base = page_at = in.t * kTile / a.c.block_size;
+            page_off = in.t * kTile - page_at * a.c.block_size;
+            pages = table_entry(in.b, in.len, page_base + lane);
+        }
+        look_ahead();
     }
     // copies: lane -> word `word` of the rows copy_row + j * kRowsPerCopy
     const int copy_row = lane / S::kWords, word = lane % S::kWords;
     auto swizzle = [](int r, int w) { return S::kWords >= 8 ? (w & ~7) | ((w ^ r) & 7) : (w ^ (r >> 1)) & 3; };
     const uint32_t copy_dst = copy_row * kRow + swizzle(copy_row, word) * 16;
+    const bool word_there = word * 16 < row_bytes, dense = a.c.st == kRow;
+    const int64_t lane_from = copy_row * a.c.st + word * 16, v_less_k = a.c.v - a.c.k;
+    const float* const lane_scale = kE4m3 ? (lane < 16 ? a.c.k_scale : a.c.v_scale) + (lane & 15) * a.c.sst : nullptr;
     auto copy_tile = [&](int stage) {
-        const uint32_t ks = smem_addr(my_ring) + stage * S::kStageBytes, vs = ks + kTile * kRow;
+        const uint32_t ks = my_ring_at + stage * S::kStageBytes, vs = ks + kTile * kRow;
         const int head = in.hc / parts, rows = in.len - in.t * kTile;             // rows that exist: at least 16, but at a sequence's end
-        const int64_t v_less_k = a.c.v - a.c.k;
-        const bool word_there = word * 16 < row_bytes;
+        auto dst_of = [&](int j) { return j * S::kRowsPerCopy * kRow + (copy_dst ^ (S::kWords >= 8 ? ((j * S::kRowsPerCopy) & 7) * 16 : 0)); };
         if (paged16) {
-            bool there = rows > 0;
-            int64_t p = page;
-            if (there && (p < 0 || p >= a.c.num_blocks)) {
-                there = false;
-                if (lane == 0) report_status(a.status, kDevBadPage);
+            if ((unsigned)(page_at - page_base) >= 32u) {
+                page_base = page_at;
+                pages = table_entry(in.b, in.len, page_base + lane);
             }
-            if (!there) p = 0;
-            const unsigned char* src = a.c.k + p * a.c.sb + (there ? page_off : 0) * a.c.st + head * a.c.sh;
+            const int64_t p = __shfl_sync(0xffffffffu, pages, page_at - page_base);
+            if (rows >= kTile && p >= 0 && p < a.c.num_blocks) {                  // a whole tile of a page
+                const unsigned char* k_row = a.c.k + p * a.c.sb + page_off * a.c.st + head * a.c.sh + lane_from;
+                const unsigned char* v_row = k_row + v_less_k;
+                if (word_there) {
+                    if (dense) {
 #pragma unroll
-            for (int j = 0; j < S::kCopies; ++j) {
-                const int r = copy_row + j * S::kRowsPerCopy;
-                const bool ok = there && r < rows && word_there;
-                const unsigned char* row = ok ? src + r * a.c.st + word * 16 : a.c.k;
-                const uint32_t dst = j * S::kRowsPerCopy * kRow + (copy_dst ^ (S::kWords >= 8 ? ((j * S::kRowsPerCopy) & 7) * 16 : 0));
-                copy16(ks + dst, row, ok);
-                copy16(vs + dst, row + v_less_k, ok);
+                        for (int j = 0; j < S::kCopies; ++j) {
+                            copy16(ks + dst_of(j), k_row + j * S::kRowsPerCopy * kRow);
+                            copy16(vs + dst_of(j), v_row + j * S::kRowsPerCopy * kRow);
+                        }
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < S::kCopies; ++j) {
+                            copy16(ks + dst_of(j), k_row);
+                            copy16(vs + dst_of(j), v_row);
+                            k_row += S::kRowsPerCopy * a.c.st;
+                            v_row += S::kRowsPerCopy * a.c.st;
+                        }
+                    }
+                }
+                if (kE4m3) copy4(vs + kTile * kRow + lane * 4, lane_scale + p * a.c.ssb + page_off * a.c.sst + head * a.c.ssh, true);
+                page_off += kTile;
+                if (page_off == a.c.block_size) { page_off = 0; ++page_at; }
+                return;
             }
-            if (kE4m3) {
-                const int r = lane & 15;
-                const bool ok = there && r < rows;
-                const float* s = (lane < 16 ? a.c.k_scale : a.c.v_scale) + (ok ? p * a.c.ssb + (int64_t)(page_off + r) * a.c.sst + head * a.c.ssh : 0);
-                copy4(vs + kTile * kRow + lane * 4, s, ok);
+        }
+        // a sequence's end, rows with pages of their own, pages that do not exist: row by row, zeros where there is none
+        const int r16 = lane & 15, token = in.t * kTile + r16;
+        bool there = r16 < rows;
+        int64_t p = 0, off = 0;
+        if (there) {
+            const int i = token / a.c.block_size;
+            off = token - (int64_t)i * a.c.block_size;
+            p = ld_dep(a.tables + (int64_t)in.b * a.ld_tables + i);
+            if (p < 0 || p >= a.c.num_blocks) {
+                there = false;
+                report_status(a.status, kDevBadPage);
             }
+        }
+        const long long row_from = there ? p * a.c.sb + off * a.c.st + head * a.c.sh : -1;
+#pragma unroll 1
+        for (int j = 0; j < S::kCopies; ++j) {
+            const long long from = __shfl_sync(0xffffffffu, row_from, copy_row + j * S::kRowsPerCopy);
+            const bool ok = from >= 0 && word_there;
+            const unsigned char* row = ok ? a.c.k + from + word * 16 : a.c.k;
+            copy16(ks + dst_of(j), row, ok);
+            copy16(vs + dst_of(j), ok ? row + v_less_k : a.c.v, ok);
+        }
+        if (kE4m3) {
+            const float* s = (lane < 16 ? a.c.k_scale : a.c.v_scale) + (there ? p * a.c.ssb + off * a.c.sst + head * a.c.ssh : 0);
+            copy4(vs + kTile * kRow + lane * 4, s, there);
+        }
+        if (paged16) {
             page_off += kTile;
             if (page_off == a.c.block_size) { page_off = 0; ++page_at; }
-        } else {                                                                  // every row has a page of its own
-            const int r16 = lane & 15, token = in.t * kTile + r16;
-            bool there = r16 < rows;
-            int64_t p = 0, off = 0;
-            if (there) {
-                const int i = token / a.c.block_size;
-                off = token - (int64_t)i * a.c.block_size;
-                p = ld_dep(a.tables + (int64_t)in.b * a.ld_tables + i);
-                if (p < 0 || p >= a.c.num_blocks) {
-                    there = false;
-                    report_status(a.status, kDevBadPage);
-                }
-            }
-            const long long mine = there ? p * a.c.sb + off * a.c.st + head * a.c.sh : -1;
-#pragma unroll
-            for (int j = 0; j < S::kCopies; ++j) {
-                const long long from = __shfl_sync(0xffffffffu, mine, copy_row + j * S::kRowsPerCopy);
-                const bool ok = from >= 0 && word_there;
-                const unsigned char* row = ok ? a.c.k + from + word * 16 : a.c.k;
-                const uint32_t dst = j * S::kRowsPerCopy * kRow + (copy_dst ^ (S::kWords >= 8 ? ((j * S::kRowsPerCopy) & 7) * 16 : 0));
-                copy16(ks + dst, row, ok);
-                copy16(vs + dst, row + v_less_k, ok);
-            }
-            if (kE4m3) {
-                const float* s = (lane < 16 ? a.c.k_scale : a.c.v_scale) + (there ? p * a.c.ssb + off * a.c.sst + head * a.c.ssh : 0);
-                copy4(vs + kTile * kRow + lane * 4, s, there);
-            }
         }
-        // on to the next tile
-        if (++in.t == in.tiles) {
-            in.t = 0;
-            page_at = page_off = 0;
-            if (++in.hc == segments) {
-                in.hc = 0;
-                ++in.b;
-                in.len = next_len;
-                in.tiles = tiles_of(in.len);
-                if (in.b + 1 < a.batch) next_len = tokens_of(a, in.b + 1, most);
-            }
-        }
+    };
+    auto next_tile = [&] {
+        if (++in.t < in.tiles) return;
+        in.t = 0;
+        page_at = page_off = 0;
+        if (++in.hc < segments) return;
+        in.hc = 0;
+        ++in.b;
+        in.len = next_len;
+        in.tiles = tiles_of(in.len);
+        pages = next_pages;
+        page_base = 0;
+        look_ahead();
     };
 
     const Result result(a);
@@ -375,7 +426,7 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
                 to_score[n][0] = to_score[n][1] = base;
             }
 #pragma unroll
-            for (int i = 0; i < 2; ++i) { m[n][i] = -INFINITY; l[n][i] = 0.f; }
+            for (int i = 0; i < 2; ++i) { m[n][i] = kNone; l[n][i] = 0.f; }
 #pragma unroll
             for (int c = 0; c < kD / 16; ++c)
 #pragma unroll
@@ -383,9 +434,12 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
         }
     };
 
-    const int mi = lane >> 3, lr = lane & 7;                                       // ldmatrix: this lane's matrix and row
+    // ldmatrix: where this lane's row of a matrix is, for the first channels; word w + its is at the same place ^ (w & 7) * 16, + (w & ~7) * 16
+    const int mi = lane >> 3, lr = lane & 7, k_r = lr + (mi & 1) * 8, v_r = kE4m3 ? k_r : lr + (mi >> 1) * 8;
+    const uint32_t k_lane = k_r * kRow + swizzle(k_r, mi >> 1) * 16, v_lane = v_r * kRow + swizzle(v_r, kE4m3 ? mi >> 1 : mi & 1) * 16;
+    auto words_on = [](uint32_t lane_at, int w) { return (lane_at ^ ((w & 7) * 16)) + (w & ~7) * 16; };
     auto work_on = [&](int stage) {
-        const uint32_t ks = smem_addr(my_ring) + stage * S::kStageBytes, vs = ks + kTile * kRow;
+        const uint32_t ks = my_ring_at + stage * S::kStageBytes, k_at = ks + k_lane, v_at = ks + kTile * kRow + v_lane;
         float s[kN][4];
 #pragma unroll
         for (int n = 0; n < kN; ++n)
@@ -393,12 +447,10 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
             for (int i = 0; i < 4; ++i) s[n][i] = 0.f;
         // scores: rows of the A operand are tokens
         {
-            const int r = lr + (mi & 1) * 8;
 #pragma unroll
             for (int c = 0; c < kD / 16; c += kE4m3 ? 2 : 1) {
                 uint32_t f[4];
-                const int w = (kE4m3 ? c : 2 * c) + (mi >> 1);
-                ldmatrix4(f, ks + r * kRow + swizzle(r, w) * 16);
+                ldmatrix4(f, words_on(k_at, kE4m3 ? c : 2 * c));
                 if (kE4m3) {
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
@@ -424,45 +476,52 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
         float top[kN][2];
         bool raised = false;
 #pragma unroll
-        for (int n = 0; n < kN; ++n) {
+        for (int n = 0; n < kN; ++n)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if (kE4m3) s[n][i] *= k_scale[i >> 1];
-                s[n][i] *= to_score[n][i & 1];
-                if (rows < kTile && g + 8 * (i >> 1) >= rows) s[n][i] = -INFINITY;
-            }
+            for (int i = 0; i < 4; ++i) s[n][i] *= kE4m3 ? k_scale[i >> 1] * to_score[n][i & 1] : to_score[n][i & 1];
+        if (rows < kTile) {
+#pragma unroll
+            for (int n = 0; n < kN; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (g + 8 * (i >> 1) >= rows) s[n][i] = -INFINITY;
+        }
+#pragma unroll
+        for (int n = 0; n < kN; ++n)
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                float x = fmaxf(s[n][i], s[n][2 + i]);
-                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
-                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
-                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-                top[n][i] = fmaxf(m[n][i], x);
-                raised |= top[n][i] != m[n][i];
+                top[n][i] = fmaxf(s[n][i], s[n][2 + i]);
+                raised |= top[n][i] > m[n][i] + kSlack;
             }
-        }
         int exp_now = value_exp;
         if (kE4m3) {
-            const uint32_t e = __reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(fabsf(v_scale[0]), fabsf(v_scale[1])))) >> 23;
-            exp_now = max(value_exp, (int)e);
+            exp_now = max(value_exp, (int)(__float_as_uint(fmaxf(fabsf(v_scale[0]), fabsf(v_scale[1]))) >> 23));
             raised |= exp_now != value_exp;
         }
         if (__any_sync(0xffffffffu, raised)) {
+            if (kE4m3) exp_now = __reduce_max_sync(0xffffffffu, exp_now);
             const float down = kE4m3 ? exp2_approx((float)(value_exp - exp_now)) : 1.f;
+            value_exp = exp_now;
 #pragma unroll
             for (int n = 0; n < kN; ++n)
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    const float f = weight_of(m[n][i], top[n][i]);
-                    m[n][i] = top[n][i];
+                    float x = top[n][i];
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+                    x = fmaxf(m[n][i], x);
+                    const float f = exp2_approx(m[n][i] - x), fd = f * down;
+                    m[n][i] = x;
                     l[n][i] *= f;
 #pragma unroll
-                    for (int c = 0; c < kD / 16; ++c) { o[c][n][i] *= f * down; o[c][n][2 + i] *= f * down; }
+                    for (int c = 0; c < kD / 16; ++c) { o[c][n][i] *= fd; o[c][n][2 + i] *= fd; }
                 }
-            value_exp = exp_now;
         }
         uint32_t hi[kN][2], lo[kN][2];
-        const float up = kE4m3 ? __uint_as_float((uint32_t)(268 - value_exp) << 23) : 1.f;    // 2^(14 - (value_exp - 127))
+        const float up = kE4m3 ? __uint_as_float((uint32_t)(260 - value_exp) << 23) : 1.f;    // 2^(6 - (value_exp - 127)): products below 2^15
+        float v_up[2] = {1.f, 1.f};
+        if (kE4m3) { v_up[0] = v_scale[0] * up; v_up[1] = v_scale[1] * up; }
 #pragma unroll
         for (int n = 0; n < kN; ++n)
 #pragma unroll
@@ -470,9 +529,9 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
                 float p[2];
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    p[i] = exp2_approx(s[n][2 * h + i] - (m[n][i] == -INFINITY ? 0.f : m[n][i]));
+                    p[i] = exp2_approx(s[n][2 * h + i] - m[n][i]);
                     l[n][i] += p[i];
-                    if (kE4m3) p[i] *= v_scale[h] * up;
+                    if (kE4m3) p[i] *= v_up[h];
                 }
                 split2<kE4m3>(p[0], p[1], hi[n][h], lo[n][h]);
                 hi[n][h] = transposed(hi[n][h]);
@@ -484,8 +543,7 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
             uint32_t f[4];
             if (kE4m3) {
                 // a lane's word holds channels 2g and 2g + 1 of two tokens: the first are row g, the second row g + 8
-                const int r = lr + (mi & 1) * 8, w = c + (mi >> 1);
-                ldmatrix4_trans(f, vs + r * kRow + swizzle(r, w) * 16);
+                ldmatrix4_trans(f, words_on(v_at, c));
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     const uint32_t x = prmt(f[2 * h], 0x3120), y = prmt(f[2 * h + 1], 0x3120);
@@ -498,8 +556,7 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
                     }
                 }
             } else {
-                const int r = lr + (mi >> 1) * 8, w = 2 * c + (mi & 1);
-                ldmatrix4_trans(f, vs + r * kRow + swizzle(r, w) * 16);
+                ldmatrix4_trans(f, words_on(v_at, 2 * c));
 #pragma unroll
                 for (int n = 0; n < kN; ++n) {
                     mma<false>(o[c][n], f[0], f[1], f[2], f[3], hi[n][0], hi[n][1]);
@@ -526,16 +583,15 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
     if (lane < 2) s_piece[2 * warp + lane].tile0 = -1;
     __syncwarp();
     int to = 0, from = 0;                                                          // stages: of the next copy, of the next tile's work
-    for (int64_t i = 1 - kStages; i < todo; ++i) {
+    for (int i = 1 - kStages; i < todo; ++i) {
         if (i >= 0) {
             copies_wait<kStages - 2>();
             __syncwarp();
         }
-        const int64_t ahead = i + kStages - 1;
-        if (ahead < todo) {
+        if (i < todo - (kStages - 1)) {
             copy_tile(to);
+            next_tile();
             to = to + 1 == kStages ? 0 : to + 1;
-            if (ahead + 1 < todo) next_page();
         }
         copies_end();
         if (i < 0) {
@@ -546,7 +602,7 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
         from = from + 1 == kStages ? 0 : from + 1;
         const bool ends = at.t + 1 == at.tiles, last = i + 1 == todo;
         if (ends || last) {
-            const float back = kE4m3 ? __uint_as_float((uint32_t)(value_exp - 14) << 23) : 1.f;
+            const float back = kE4m3 ? __uint_as_float((uint32_t)(value_exp - 6) << 23) : 1.f;
 #pragma unroll
             for (int n = 0; n < kN; ++n)
 #pragma unroll
@@ -610,13 +666,17 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
             const int run = __popc(upto) - 1;
             s_first[run] = __popc(below);
             if (run == runs - 1) s_first[runs] = __popc(there);
-            if (p.tile0 < cta0) s_open[0] = run;
-            else if (p.tile0 + p.tiles > cta1) s_open[1] = run;
+            if (p.tile0 < cta0 || p.tile0 + p.tiles > cta1) {
+                const int w = p.tile0 < cta0 ? 0 : 1, c0 = share_of(total, ctas, p.tile0);
+                s_open[w] = run;
+                s_cta0[w] = c0;
+                s_ctas[w] = share_of(total, ctas, p.tile0 + p.tiles - 1) - c0 + 1;
+            }
         }
     }
     // the weights of a run's pieces, a warp for a query head
     for (int col = warp; col < kHeads; col += kWarps) {
-        const float pm = seg >= 0 ? s_m[lane][col] : -INFINITY;
+        const float pm = seg >= 0 ? s_m[lane][col] : kNone;
         float top = pm, sum;
 #pragma unroll
         for (int x = 1; x < 32; x <<= 1) {
@@ -624,7 +684,7 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
             if (lane - x >= first) top = fmaxf(top, y);
         }
         top = __shfl_sync(0xffffffffu, top, end - 1);
-        const float f = weight_of(pm, top);
+        const float f = exp2_approx(pm - top);
         sum = seg >= 0 ? f * s_l[lane][col] : 0.f;
 #pragma unroll
         for (int x = 1; x < 32; x <<= 1) {
@@ -675,12 +735,8 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
     if (tid < 2) {
         bool last = false;
         if (s_open[tid] >= 0) {
-            const Piece p = s_piece[s_entry[s_first[s_open[tid]]]];
-            const int c0 = share_of(total, ctas, p.tile0), c1 = share_of(total, ctas, p.tile0 + p.tiles - 1);
-            __threadfence();
-            last = atomicAdd(a.counters + c0, 1) == c1 - c0;
-            if (last) a.counters[c0] = 0;                                          // for the next call
-            __threadfence();
+            last = arrive(a.counters + s_cta0[tid]) == s_ctas[tid] - 1;
+            if (last) a.counters[s_cta0[tid]] = 0;                                 // for the next call
         }
         s_last[tid] = last;
     }
@@ -689,13 +745,13 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
     for (int w = 0; w < 2; ++w) {
         if (!s_last[w]) continue;
         const Piece p = s_piece[s_entry[s_first[s_open[w]]]];
-        const int c0 = share_of(total, ctas, p.tile0), count = share_of(total, ctas, p.tile0 + p.tiles - 1) - c0 + 1;
+        const int c0 = s_cta0[w], count = s_ctas[w];
         auto piece_of = [&](int i) { return pieces + ((int64_t)(c0 + i) * 2 + (i == 0)) * kOut; };
         for (int col = warp; col < kHeads; col += kWarps) {                        // a warp for a query head, a lane for a few CTAs
-            float pm[kMaxCtas / 32], pl[kMaxCtas / 32], top = -INFINITY, sum = 0.f;
+            float pm[kMaxCtas / 32], pl[kMaxCtas / 32], top = kNone, sum = 0.f;
 #pragma unroll
             for (int i = 0; i < kMaxCtas / 32; ++i) {
-                pm[i] = -INFINITY;
+                pm[i] = kNone;
                 pl[i] = 0.f;
                 if (i * 32 + lane < count) {
                     pm[i] = ld_dep_l2(piece_of(i * 32 + lane) + kPiece + col);
@@ -706,7 +762,7 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
             for (int x = 16; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
 #pragma unroll
             for (int i = 0; i < kMaxCtas / 32; ++i) {
-                const float f = weight_of(pm[i], top);
+                const float f = exp2_approx(pm[i] - top);
                 sum += f * pl[i];
                 if (i * 32 + lane < count) s_share[i * 32 + lane][col] = f;
             }
