@@ -51,7 +51,7 @@ struct Shape {
     static constexpr int kStageBytes = 2 * kTile * kRow + (kE4m3 ? 2 * kTile * 4 : 0);
     static constexpr int kRing = kWarps * kStages * kStageBytes;
     static constexpr int kPiece = kHeads * kD;                            // floats of a piece's sums
-    static constexpr int kSmem = kRing > kWarps * kPiece * 4 ? kRing : kWarps * kPiece * 4;
+    static_assert(kPiece * 4 <= kStages * kStageBytes, "a warp's sums lie in its ring");
     static_assert(kWords <= 32, "a row is one copy instruction of a warp at most");
 };
 
@@ -99,6 +99,16 @@ constexpr float kNone = -3.402823466e38f;
 // Weights are relative to a score that is at most 2^kSlack below the largest: it follows the maximum only where that
 // runs away from it, so that the sums are rescaled once or twice per segment and not with every new maximum.
 constexpr float kSlack = 8.f;
+__device__ __forceinline__ float warp_max(float x) {
+    float r;
+    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ float reciprocal(float x) {
+    float r;
+    asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
 __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&h);
@@ -142,7 +152,7 @@ __device__ __forceinline__ int share_of(int64_t total, int parts, int64_t tile) 
 
 struct Piece {                  // part of a segment
     int64_t tile0;              // the segment's first tile in the list, -1: none
-    int tiles, b, hc;           // its tiles, sequence, key head and part of its query heads
+    int tiles, b, head0, heads; // its tiles, sequence and query heads
 };
 
 // Where results go: bf16, or the codes of the bf16 value.
@@ -192,8 +202,8 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
     __shared__ Piece s_piece[2 * kWarps];
     // (read two heads at a time)
     __shared__ __align__(16) float s_m[2 * kWarps][kHeads], s_l[2 * kWarps][kHeads], s_f[2 * kWarps][kHeads], s_inv[kHeads], s_share[kMaxCtas][kHeads];
-    __shared__ int s_entry[2 * kWarps], s_first[2 * kWarps + 1];                 // the pieces that there are, and where a run of one segment's begins
-    __shared__ int s_open[2], s_last[2], s_cta0[2], s_ctas[2];                   // runs that other CTAs have pieces of; which CTAs
+    __shared__ int s_entry[2 * kWarps];                                          // the pieces that there are, in the order of the list
+    __shared__ int s_last[2], s_cta0[2], s_ctas[2];                              // segments that other CTAs have pieces of; which CTAs
 
     pdl_launch_dependents();
     pdl_wait();
@@ -204,12 +214,14 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
     // ---- shares: every warp for itself, a lane for a stretch of sequences -------------------------------------------
     const int stretch = (a.batch + 31) >> 5, lane_b = lane * stretch;
     int64_t mine = 0;
+    int lane_len = 0;                                                             // of the stretch's last
 #pragma unroll 8
     for (int i = 0; i < stretch; ++i) {
         if (lane_b + i < a.batch) {
             const int len = ld_dep(a.lens + lane_b + i);
             if (len > most && blockIdx.x == 0) report_status(a.status, kDevBadPage);
-            mine += tiles_of(len < most ? len : (int)most);
+            lane_len = len < 0 ? 0 : len < most ? len : (int)most;
+            mine += tiles_of(lane_len);
         }
     }
     mine *= segments;
@@ -228,7 +240,6 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
     const int64_t cta0 = share_begin(total, ctas, blockIdx.x), cta1 = share_begin(total, ctas, blockIdx.x + 1);
     const int64_t begin = cta0 + (cta1 - cta0) * warp / kWarps, todo64 = cta0 + (cta1 - cta0) * (warp + 1) / kWarps - begin;
     const int todo = (int)(todo64 < 0x7fffffff ? todo64 : 0x7fffffff);
-    if (tid < 2) s_open[tid] = -1;
 
     // ---- a warp's tiles -----------------------------------------------------------------------------------------------
     unsigned char* const my_ring = ring + warp * (kStages * S::kStageBytes);
@@ -241,23 +252,37 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
         __syncwarp();
     }
 
-    struct Place { int b, hc, t, len, tiles; } in, at;              // of the next tile to copy, and to work on
+    struct Place {
+        int b, head, part, t, len, tiles;                           // sequence, key head, part of its query heads, tile
+    } in, at;                                                       // of the next tile to copy, and to work on
+    auto next_segment = [&](Place& x) {                             // whether it is one of the same sequence
+        if (++x.part < parts) return true;
+        x.part = 0;
+        if (++x.head < a.c.kv_heads) return true;
+        x.head = 0;
+        ++x.b;
+        return false;
+    };
     // Pages of `in` where they hold whole tiles: 32 entries of its table at a time, a lane each, from page_base on
-    int next_len = 0, pages = 0, next_pages = 0, page_base = 0, page_at = 0, page_off = 0;
+    int pages = 0, page_base = 0, page_at = 0, page_off = 0;
+    int next_b = -1, next_len = 0, next_pages = 0;                  // the sequence behind it, once it was looked at
     auto table_entry = [&](int b, int len, int i) {
         return (int64_t)i * a.c.block_size < len ? ld_dep(a.tables + (int64_t)b * a.ld_tables + i) : 0;
     };
-    auto look_ahead = [&] {
-        if (in.b + 1 < a.batch) {
-            next_len = tokens_of(a, in.b + 1, most);
-            if (paged16) next_pages = table_entry(in.b + 1, next_len, lane);
+    auto look_at = [&](int b) {
+        next_b = b;
+        if (b < a.batch) {
+            next_len = tokens_of(a, b, most);
+            if (paged16) next_pages = table_entry(b, next_len, lane);
         }
     };
     if (todo > 0) {
         int64_t inside = begin - before;
         const int where = __ffs(__ballot_sync(0xffffffffu, inside >= 0 && inside < mine)) - 1;
         inside = __shfl_sync(0xffffffffu, inside, where);
-        for (int b0 = where * stretch;; b0 += 32) {                               // (it is one of the stretch's)
+        in.b = where;
+        in.len = __shfl_sync(0xffffffffu, lane_len, where);
+        if (stretch > 1) for (int b0 = where * stretch;; b0 += 32) {              // (it is one of the stretch's)
             const int len = b0 + lane < a.batch ? tokens_of(a, b0 + lane, most) : 0;
             const int64_t all = b0 + lane < a.batch ? (int64_t)tiles_of(len) * segments : 0;
             int64_t upto = all;
@@ -277,15 +302,16 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
             inside -= __shfl_sync(0xffffffffu, upto, 31);
         }
         in.tiles = tiles_of(in.len);
-        in.hc = (int)quotient(inside, in.tiles);
-        in.t = (int)(inside - (int64_t)in.hc * in.tiles);
+        const int segment = (int)quotient(inside, in.tiles);
+        in.t = (int)(inside - (int64_t)segment * in.tiles);
+        in.head = parts == 1 ? segment : segment / parts;
+        in.part = segment - in.head * parts;
         at = in;
         if (paged16) {
             page_base = page_at = in.t * kTile / a.c.block_size;
             page_off = in.t * kTile - page_at * a.c.block_size;
             pages = table_entry(in.b, in.len, page_base + lane);
         }
-        look_ahead();
     }
     // copies: lane -> word `word` of the rows copy_row + j * kRowsPerCopy
     const int copy_row = lane / S::kWords, word = lane % S::kWords;
@@ -296,7 +322,7 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
     const float* const lane_scale = kE4m3 ? (lane < 16 ? a.c.k_scale : a.c.v_scale) + (lane & 15) * a.c.sst : nullptr;
     auto copy_tile = [&](int stage) {
         const uint32_t ks = my_ring_at + stage * S::kStageBytes, vs = ks + kTile * kRow;
-        const int head = in.hc / parts, rows = in.len - in.t * kTile;             // rows that exist: at least 16, but at a sequence's end
+        const int head = in.head, rows = in.len - in.t * kTile;                   // rows that exist: at least 16, but at a sequence's end
         auto dst_of = [&](int j) { return j * S::kRowsPerCopy * kRow + (copy_dst ^ (S::kWords >= 8 ? ((j * S::kRowsPerCopy) & 7) * 16 : 0)); };
         if (paged16) {
             if ((unsigned)(page_at - page_base) >= 32u) {
@@ -365,14 +391,13 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
         if (++in.t < in.tiles) return;
         in.t = 0;
         page_at = page_off = 0;
-        if (++in.hc < segments) return;
-        in.hc = 0;
-        ++in.b;
+        if (next_segment(in)) return;
+        if (next_b != in.b) look_at(in.b);
         in.len = next_len;
         in.tiles = tiles_of(in.len);
         pages = next_pages;
         page_base = 0;
-        look_ahead();
+        look_at(in.b + 1);
     };
 
     const Result result(a);
@@ -380,7 +405,7 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
     float o[kD / 16][kN][4], m[kN][2], l[kN][2], to_score[kN][2];
     int value_exp = 15;                                                            // exponent field that the values' scales are relative to
     auto begin_segment = [&] {
-        const int part = at.hc % parts, head0 = at.hc / parts * group + part * kHeads, heads = min(kHeads, group - part * kHeads);
+        const int head0 = at.head * group + at.part * kHeads, heads = min(kHeads, group - at.part * kHeads);
         value_exp = 15;
 #pragma unroll
         for (int n = 0; n < kN; ++n) {
@@ -595,7 +620,10 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
         }
         copies_end();
         if (i < 0) {
-            if (i == -1 && todo > 0) begin_segment();
+            if (i == -1 && todo > 0) {
+                begin_segment();
+                if (next_b < 0) look_at(in.b + 1);
+            }
             continue;
         }
         work_on(from);
@@ -615,30 +643,26 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
                         for (int c = 0; c < kD / 16; ++c) { o[c][n][j] *= back; o[c][n][2 + j] *= back; }
                 }
             if (ends && i >= at.t) {                                               // the whole segment was this warp's
-                const int part = at.hc % parts;
 #pragma unroll
                 for (int n = 0; n < kN; ++n) {
-                    const float2 inv = at.len > 0 ? float2{__fdiv_rn(1.f, l[n][0]), __fdiv_rn(1.f, l[n][1])} : float2{0.f, 0.f};
+                    const float2 inv = at.len > 0 ? float2{reciprocal(l[n][0]), reciprocal(l[n][1])} : float2{0.f, 0.f};
 #pragma unroll
                     for (int c = 0; c < kD / 16; ++c)
-                        result.store<kE4m3>(at.b, at.hc / parts * group + part * kHeads, min(kHeads, group - part * kHeads), c, n,
+                        result.store<kE4m3>(at.b, at.head * group + at.part * kHeads, min(kHeads, group - at.part * kHeads), c, n,
                                             {o[c][n][0], o[c][n][1], o[c][n][2], o[c][n][3]}, inv);
                 }
             } else {
-                if (lane == 0) s_piece[2 * warp + last] = {begin + i - at.t, at.tiles, at.b, at.hc};
+                if (lane == 0)
+                    s_piece[2 * warp + last] = {begin + i - at.t, at.tiles, at.b, at.head * group + at.part * kHeads, min(kHeads, group - at.part * kHeads)};
                 if (last) kept = true;                                             // stays in registers until the rings are done with
                 else keep_piece(false, early);
             }
         }
         if (++at.t == at.tiles) {
             at.t = 0;
-            if (++at.hc == segments) {
-                at.hc = 0;
-                ++at.b;
-                if (i + 1 < todo) {
-                    at.len = tokens_of(a, at.b, most);
-                    at.tiles = tiles_of(at.len);
-                }
+            if (!next_segment(at) && i + 1 < todo) {
+                at.len = tokens_of(a, at.b, most);
+                at.tiles = tiles_of(at.len);
             }
             if (i + 1 < todo) begin_segment();
         }
@@ -646,97 +670,85 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
 
     // ---- pieces of a segment in this CTA ------------------------------------------------------------------------------
     copies_wait<0>();
-    __syncthreads();
-    float* const sums = reinterpret_cast<float*>(ring);                            // [warp][piece], over the rings
-    if (kept) keep_piece(true, sums + warp * kPiece);
+    __syncwarp();
+    if (kept) keep_piece(true, reinterpret_cast<float*>(my_ring));
     __syncthreads();
     // A lane for a piece (two per warp, the second its last), every warp for itself: runs of pieces of one segment.
-    const int64_t seg = lane < 2 * kWarps ? s_piece[lane].tile0 : -1;
+    const int64_t seg = lane < 2 * kWarps ? s_piece[lane].tile0 : -1, seg_end = seg + (lane < 2 * kWarps ? s_piece[lane].tiles : 0);
     const uint32_t there = __ballot_sync(0xffffffffu, seg >= 0), below = there & ((1u << lane) - 1);
     const int64_t prev = __shfl_sync(0xffffffffu, seg, below ? 31 - __clz(below) : lane);
-    const uint32_t firsts = __ballot_sync(0xffffffffu, seg >= 0 && (below == 0 || prev != seg));
-    if (firsts == 0) return;
-    const int runs = __popc(firsts);
-    const uint32_t upto = firsts & ((2u << lane) - 1), beyond = firsts & ~((2u << lane) - 1);
-    const int first = upto ? 31 - __clz(upto) : 0, end = beyond ? __ffs(beyond) - 1 : 32;      // lanes of this lane's run
-    if (warp == 0 && seg >= 0) {
-        s_entry[__popc(below)] = lane;
-        if (lane == first) {
-            const Piece p = s_piece[lane];
-            const int run = __popc(upto) - 1;
-            s_first[run] = __popc(below);
-            if (run == runs - 1) s_first[runs] = __popc(there);
-            if (p.tile0 < cta0 || p.tile0 + p.tiles > cta1) {
-                const int w = p.tile0 < cta0 ? 0 : 1, c0 = share_of(total, ctas, p.tile0);
-                s_open[w] = run;
-                s_cta0[w] = c0;
-                s_ctas[w] = share_of(total, ctas, p.tile0 + p.tiles - 1) - c0 + 1;
-            }
-        }
-    }
-    // the weights of a run's pieces, a warp for a query head
-    for (int col = warp; col < kHeads; col += kWarps) {
-        const float pm = seg >= 0 ? s_m[lane][col] : kNone;
-        float top = pm, sum;
-#pragma unroll
-        for (int x = 1; x < 32; x <<= 1) {
-            const float y = __shfl_up_sync(0xffffffffu, top, x);
-            if (lane - x >= first) top = fmaxf(top, y);
-        }
-        top = __shfl_sync(0xffffffffu, top, end - 1);
-        const float f = exp2_approx(pm - top);
-        sum = seg >= 0 ? f * s_l[lane][col] : 0.f;
-#pragma unroll
-        for (int x = 1; x < 32; x <<= 1) {
-            const float y = __shfl_up_sync(0xffffffffu, sum, x);
-            if (lane - x >= first) sum += y;
-        }
-        sum = __shfl_sync(0xffffffffu, sum, end - 1);
-        if (seg >= 0) {
-            s_f[lane][col] = f;
-            if (lane == first) { s_m[lane][col] = top; s_l[lane][col] = sum; }     // (this lane's alone from here on)
-        }
-    }
-    __syncthreads();
+    const bool first = seg >= 0 && (below == 0 || prev != seg);
+    const uint32_t firsts = __ballot_sync(0xffffffffu, first);
+    // ... and the one that other CTAs began, the one that others go on with
+    const uint32_t open0 = __ballot_sync(0xffffffffu, first && seg < cta0), open1 = __ballot_sync(0xffffffffu, first && seg >= cta0 && seg_end > cta1);
     constexpr int kUnits = kPiece / 4;                                             // fragments of a lane: two heads, two channels
     constexpr int kOut = kPiece + 2 * kHeads;
     float* const pieces = a.partial + (int64_t)gridDim.x * kWarps * kPiece;         // [CTA][2][sums | m | l]
-    for (int x = tid; x < runs * kUnits; x += S::kThreads) {
-        const int run = x / kUnits, unit = x % kUnits, col = (unit >> 5) % kN * 8 + 2 * t4;
-        const int e0 = s_entry[s_first[run]];
+    if (warp == 0 && seg >= 0) s_entry[__popc(below)] = lane;
+    // the weights of a run's pieces, and their part of its sum of weights: a warp for a query head
+    for (int col = warp; col < kHeads; col += kWarps) {
+        const float pm = seg >= 0 ? s_m[lane][col] : kNone, pl = seg >= 0 ? s_l[lane][col] : 0.f;
+        float top = kNone;
+        for (uint32_t left = firsts; left; left &= left - 1) {
+            const uint32_t rest = left & (left - 1), members = there & (0u - (left & (0u - left))) & (rest ? (rest & (0u - rest)) - 1 : 0xffffffffu);
+            const bool in_run = members >> lane & 1;
+            const float t = warp_max(in_run ? pm : kNone);
+            if (in_run) top = t;
+        }
+        if (seg >= 0) {
+            const float f = exp2_approx(pm - top);
+            s_f[lane][col] = f;
+            s_l[lane][col] = f * pl;
+            s_m[lane][col] = top;
+        }
+    }
+    __syncthreads();
+    uint32_t left = firsts;
+    int run = 0;
+#pragma unroll 1
+    for (int x = warp; x < __popc(firsts) * (kUnits / 32); x += kWarps) {          // a warp for the fragments of 16 channels and 8 heads
+        for (; run < x / (kUnits / 32); ++run) left &= left - 1;
+        const int at_first = __ffs(left) - 1, frag = x % (kUnits / 32), n = frag % kN, col = n * 8 + 2 * t4;
+        const uint32_t rest = left & (left - 1), members = there & ~((1u << at_first) - 1) & (rest ? (rest & (0u - rest)) - 1 : 0xffffffffu);
+        const int k0 = __popc(there & ((1u << at_first) - 1)), k1 = k0 + __popc(members);
+        float2 sum = {0.f, 0.f};
         float4 v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-        for (int k = s_first[run]; k < s_first[run + 1]; ++k) {
+        for (int k = k0; k < k1; ++k) {
             const int e = s_entry[k];
-            const float2 f = *reinterpret_cast<const float2*>(&s_f[e][col]);
-            const float* from = (e & 1) ? sums + (e >> 1) * kPiece : a.partial + ((int64_t)blockIdx.x * kWarps + (e >> 1)) * kPiece;
-            const float4 w = reinterpret_cast<const float4*>(from)[unit];
+            const float2 f = *reinterpret_cast<const float2*>(&s_f[e][col]), pl = *reinterpret_cast<const float2*>(&s_l[e][col]);
+            const float* from = (e & 1) ? reinterpret_cast<const float*>(ring + (e >> 1) * (kStages * S::kStageBytes))
+                                        : a.partial + ((int64_t)blockIdx.x * kWarps + (e >> 1)) * kPiece;
+            const float4 w = reinterpret_cast<const float4*>(from)[frag * 32 + lane];
+            sum.x += pl.x; sum.y += pl.y;
             v.x += f.x * w.x; v.y += f.y * w.y; v.z += f.x * w.z; v.w += f.y * w.w;
         }
-        const float2 sum = *reinterpret_cast<const float2*>(&s_l[e0][col]);
-        if (run == s_open[0] || run == s_open[1]) {
-            float* out = pieces + ((int64_t)blockIdx.x * 2 + (run == s_open[1])) * kOut;
-            reinterpret_cast<float4*>(out)[unit] = v;
-            if (unit >> 5 < kN && g == 0) {                                        // (the first channels' fragments have every head once)
-                *reinterpret_cast<float2*>(out + kPiece + col) = *reinterpret_cast<const float2*>(&s_m[e0][col]);
+        const uint32_t bit = 1u << at_first;
+        if ((open0 | open1) & bit) {
+            float* out = pieces + ((int64_t)blockIdx.x * 2 + (open1 & bit ? 1 : 0)) * kOut;
+            reinterpret_cast<float4*>(out)[frag * 32 + lane] = v;
+            if (frag < kN && g == 0) {                                             // (the first channels' fragments have every head once)
+                *reinterpret_cast<float2*>(out + kPiece + col) = *reinterpret_cast<const float2*>(&s_m[at_first][col]);
                 *reinterpret_cast<float2*>(out + kPiece + kHeads + col) = sum;
             }
         } else {
-            const Piece p = s_piece[e0];
-            const int part = p.hc % parts;
-            result.store<kE4m3>(p.b, p.hc / parts * group + part * kHeads, min(kHeads, group - part * kHeads), (unit >> 5) / kN, (unit >> 5) % kN, v,
-                                {__fdiv_rn(1.f, sum.x), __fdiv_rn(1.f, sum.y)});
+            const Piece p = s_piece[at_first];
+            result.store<kE4m3>(p.b, p.head0, p.heads, frag / kN, n, v, {reciprocal(sum.x), reciprocal(sum.y)});
         }
     }
 
     // ---- segments that other CTAs have pieces of: the last one to come joins them --------------------------------------
-    if (s_open[0] < 0 && s_open[1] < 0) return;
+    if ((open0 | open1) == 0) return;
     __syncthreads();
     if (tid < 2) {
         bool last = false;
-        if (s_open[tid] >= 0) {
-            last = arrive(a.counters + s_cta0[tid]) == s_ctas[tid] - 1;
-            if (last) a.counters[s_cta0[tid]] = 0;                                 // for the next call
+        if (tid == 0 ? open0 : open1) {
+            const Piece p = s_piece[__ffs(tid == 0 ? open0 : open1) - 1];
+            const int c0 = share_of(total, ctas, p.tile0), count = share_of(total, ctas, p.tile0 + p.tiles - 1) - c0 + 1;
+            s_cta0[tid] = c0;
+            s_ctas[tid] = count;
+            last = arrive(a.counters + c0) == count - 1;
+            if (last) a.counters[c0] = 0;                                          // for the next call
         }
         s_last[tid] = last;
     }
@@ -744,59 +756,82 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
 #pragma unroll 1
     for (int w = 0; w < 2; ++w) {
         if (!s_last[w]) continue;
-        const Piece p = s_piece[s_entry[s_first[s_open[w]]]];
+        const Piece p = s_piece[__ffs(w == 0 ? open0 : open1) - 1];
         const int c0 = s_cta0[w], count = s_ctas[w];
         auto piece_of = [&](int i) { return pieces + ((int64_t)(c0 + i) * 2 + (i == 0)) * kOut; };
-        for (int col = warp; col < kHeads; col += kWarps) {                        // a warp for a query head, a lane for a few CTAs
-            float pm[kMaxCtas / 32], pl[kMaxCtas / 32], top = kNone, sum = 0.f;
+        // kSlices threads share a fragment's pieces; as many pieces as the rings hold are on their way at a time
+        constexpr int kSlices = S::kThreads > kUnits ? S::kThreads / kUnits : 1, kPerThread = kUnits > S::kThreads ? kUnits / S::kThreads : 1;
+        constexpr int kAtOnce = S::kRing / (kPiece * 4);
+        const float4* const shelf = reinterpret_cast<const float4*>(ring);
+        const int slice = tid / kUnits;
+        float4 v[kPerThread];
 #pragma unroll
-            for (int i = 0; i < kMaxCtas / 32; ++i) {
-                pm[i] = kNone;
-                pl[i] = 0.f;
-                if (i * 32 + lane < count) {
-                    pm[i] = ld_dep_l2(piece_of(i * 32 + lane) + kPiece + col);
-                    pl[i] = ld_dep_l2(piece_of(i * 32 + lane) + kPiece + kHeads + col);
+        for (int k = 0; k < kPerThread; ++k) v[k] = {0.f, 0.f, 0.f, 0.f};
+        for (int i0 = 0; i0 < count; i0 += kAtOnce) {
+            const int here = count - i0 < kAtOnce ? count - i0 : kAtOnce;
+            for (int x = tid; x < here * kUnits; x += S::kThreads)
+                copy16(smem_addr(shelf + x), reinterpret_cast<const float4*>(piece_of(i0 + x / kUnits)) + x % kUnits);
+            copies_end();
+            if (i0 == 0) {
+                for (int col = warp; col < kHeads; col += kWarps) {                // a warp for a query head, a lane for a few CTAs
+                    float pm[kMaxCtas / 32], pl[kMaxCtas / 32], top = kNone, sum = 0.f;
+#pragma unroll
+                    for (int i = 0; i < kMaxCtas / 32; ++i) {
+                        pm[i] = kNone;
+                        pl[i] = 0.f;
+                        if (i * 32 + lane < count) {
+                            pm[i] = ld_dep_l2(piece_of(i * 32 + lane) + kPiece + col);
+                            pl[i] = ld_dep_l2(piece_of(i * 32 + lane) + kPiece + kHeads + col);
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < kMaxCtas / 32; ++i) top = fmaxf(top, pm[i]);
+                    for (int x = 16; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+#pragma unroll
+                    for (int i = 0; i < kMaxCtas / 32; ++i) {
+                        const float f = exp2_approx(pm[i] - top);
+                        sum += f * pl[i];
+                        if (i * 32 + lane < count) s_share[i * 32 + lane][col] = f;
+                    }
+                    for (int x = 16; x; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+                    if (lane == 0) s_inv[col] = reciprocal(sum);
                 }
-                top = fmaxf(top, pm[i]);
             }
-            for (int x = 16; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+            copies_wait<0>();
+            __syncthreads();
 #pragma unroll
-            for (int i = 0; i < kMaxCtas / 32; ++i) {
-                const float f = exp2_approx(pm[i] - top);
-                sum += f * pl[i];
-                if (i * 32 + lane < count) s_share[i * 32 + lane][col] = f;
+            for (int k = 0; k < kPerThread; ++k) {
+                const int unit = (tid + k * S::kThreads) % kUnits, col = (unit >> 5) % kN * 8 + 2 * t4;
+#pragma unroll 4
+                for (int i = slice; i < here; i += kSlices) {
+                    const float4 y = shelf[i * kUnits + unit];
+                    const float2 f = *reinterpret_cast<const float2*>(&s_share[i0 + i][col]);
+                    v[k].x += f.x * y.x; v[k].y += f.y * y.y; v[k].z += f.x * y.z; v[k].w += f.y * y.w;
+                }
             }
-            for (int x = 16; x; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
-            if (lane == 0) s_inv[col] = __fdiv_rn(1.f, sum);
+            __syncthreads();
         }
-        __syncthreads();
-        // kSlices threads share a fragment's pieces
-        constexpr int kSlices = S::kThreads > kUnits ? S::kThreads / kUnits : 1;
-        for (int x = tid; x < kSlices * kUnits; x += S::kThreads) {
-            const int unit = x % kUnits, slice = x / kUnits, n = (unit >> 5) % kN, col = n * 8 + 2 * t4;
-            float4 v = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 8
-            for (int i = slice; i < count; i += kSlices) {
-                const uint4 raw = ld_dep_l2(reinterpret_cast<const uint4*>(piece_of(i)) + unit);
-                const float2 f = *reinterpret_cast<const float2*>(&s_share[i][col]);
-                v.x += f.x * __uint_as_float(raw.x); v.y += f.y * __uint_as_float(raw.y);
-                v.z += f.x * __uint_as_float(raw.z); v.w += f.y * __uint_as_float(raw.w);
-            }
-            if (kSlices > 1) {
-                if (slice > 0) reinterpret_cast<float4*>(sums)[(slice - 1) * kUnits + unit] = v;
-                __syncthreads();                                                   // (one turn for every thread)
-                if (slice > 0) continue;
+        if (kSlices > 1) {
+            float4* const sums = reinterpret_cast<float4*>(ring);
+            if (slice > 0) sums[tid - kUnits] = v[0];
+            __syncthreads();
+            if (slice == 0) {
 #pragma unroll
                 for (int k = 1; k < kSlices; ++k) {
-                    const float4 y = reinterpret_cast<const float4*>(sums)[(k - 1) * kUnits + unit];
-                    v.x += y.x; v.y += y.y; v.z += y.z; v.w += y.w;
+                    const float4 y = sums[(k - 1) * kUnits + tid];
+                    v[0].x += y.x; v[0].y += y.y; v[0].z += y.z; v[0].w += y.w;
                 }
             }
-            const int part = p.hc % parts;
-            result.store<kE4m3>(p.b, p.hc / parts * group + part * kHeads, min(kHeads, group - part * kHeads), (unit >> 5) / kN, n, v,
-                                *reinterpret_cast<const float2*>(&s_inv[col]));
         }
-        __syncthreads();                                                           // s_share, s_inv and the sums are free again
+        if (slice == 0) {
+#pragma unroll
+            for (int k = 0; k < kPerThread; ++k) {
+                const int frag = (tid + k * S::kThreads) >> 5, n = frag % kN;
+                result.store<kE4m3>(p.b, p.head0, p.heads, frag / kN, n, v[k],
+                                    *reinterpret_cast<const float2*>(&s_inv[n * 8 + 2 * t4]));
+            }
+        }
+        __syncthreads();                                                           // s_share, s_inv and the rings are free again
     }
 }
 
@@ -810,14 +845,14 @@ cudaError_t launch(const AttnArgs& a, int group, int parts, cudaStream_t stream)
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     if (dev >= 64 || !(ready.load(std::memory_order_acquire) >> dev & 1)) {
-        e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
+        e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kRing);
         if (e != cudaSuccess) return e;
         if (dev < 64) ready.fetch_or(1ull << dev, std::memory_order_release);
     }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)attention_ctas());
     cfg.blockDim = dim3(S::kThreads);
-    cfg.dynamicSmemBytes = S::kSmem;
+    cfg.dynamicSmemBytes = S::kRing;
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     cfg.numAttrs = pdl_attribute(attr);
