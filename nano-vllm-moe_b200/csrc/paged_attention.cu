@@ -31,23 +31,25 @@
 namespace fp8lin {
 namespace {
 
-constexpr int kTile = 16;                       // tokens
+constexpr int kBlock = 16;                      // tokens of a matrix instruction
 constexpr int kMaxCtas = 192;                   // of a launch: one per SM
 constexpr float kLog2e = 1.4426950408889634f;
 
-template <bool kE4m3_, int kD_, int kN_, int kWarps_, int kStages_>
+template <bool kE4m3_, int kD_, int kN_, int kM_, int kWarps_, int kStages_>
 struct Shape {
     static constexpr bool kE4m3 = kE4m3_;
     static constexpr int kD = kD_;              // channels in shared memory: head_dim rounded up, zeros behind it
     static constexpr int kN = kN_;              // groups of 8 query heads
     static constexpr int kHeads = 8 * kN;
+    static constexpr int kM = kM_;              // blocks of 16 tokens in a tile
+    static constexpr int kTile = kBlock * kM;
     static constexpr int kWarps = kWarps_;
     static constexpr int kStages = kStages_;
     static constexpr int kThreads = 32 * kWarps;
     static constexpr int kRow = kD * (kE4m3 ? 1 : 2);                     // bytes of a row
     static constexpr int kWords = kRow / 16;                              // 16-byte words of a row
     static constexpr int kRowsPerCopy = kWords >= 32 ? 1 : 32 / kWords;   // rows that a warp's copy instruction takes
-    static constexpr int kCopies = kTile / kRowsPerCopy;
+    static constexpr int kCopies = kBlock / kRowsPerCopy;
     static constexpr int kStageBytes = 2 * kTile * kRow + (kE4m3 ? 2 * kTile * 4 : 0);
     static constexpr int kRing = kWarps * kStages * kStageBytes;
     static constexpr int kPiece = kHeads * kD;                            // floats of a piece's sums
@@ -65,6 +67,7 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
 __device__ __forceinline__ void copy4(uint32_t dst, const void* src, bool there) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(there ? 4 : 0) : "memory");
 }
+__device__ __forceinline__ void prefetch_l1(const void* p) { asm volatile("prefetch.global.L1 [%0];" ::"l"(p)); }
 __device__ __forceinline__ void copies_end() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int kLeft>
 __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory"); }
@@ -83,10 +86,10 @@ __device__ __forceinline__ uint32_t transposed(uint32_t a) {              // of 
 template <bool kF16>
 __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     if (kF16)
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
     else
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ float exp2_approx(float x) {
@@ -112,6 +115,11 @@ __device__ __forceinline__ float reciprocal(float x) {
 __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&h);
+}
+// Four e4m3 codes to f16: the lower two, the upper two.
+__device__ __forceinline__ void widen(uint32_t w, uint32_t& lo, uint32_t& hi) {
+    lo = cvt_e4m3x2_to_f16x2((uint16_t)w);
+    hi = cvt_e4m3x2_to_f16x2((uint16_t)(w >> 16));
 }
 __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t sel) { return __byte_perm(a, 0, sel); }
 
@@ -140,7 +148,8 @@ __device__ __forceinline__ int tokens_of(const AttnArgs& a, int64_t b, int64_t m
     const int len = ld_dep(a.lens + b);
     return len < 0 ? 0 : (int64_t)len > most ? (int)most : len;
 }
-__device__ __forceinline__ int tiles_of(int len) { return len > kTile ? (int)(((unsigned)len + kTile - 1) / kTile) : 1; }
+template <int kTile>
+__device__ __forceinline__ int tiles_in(int len) { return len > kTile ? (int)(((unsigned)len + kTile - 1) / kTile) : 1; }
 
 // (a division of 64 bits is a hundred instructions, on the way of every call)
 __device__ __forceinline__ int64_t quotient(int64_t n, int64_t d) {
@@ -197,7 +206,7 @@ template <class S>
 __global__ void __launch_bounds__(S::kThreads, 1)
 paged_attention_kernel(AttnArgs a, int group, int parts) {
     constexpr bool kE4m3 = S::kE4m3;
-    constexpr int kD = S::kD, kN = S::kN, kHeads = S::kHeads, kWarps = S::kWarps, kStages = S::kStages, kRow = S::kRow, kPiece = S::kPiece;
+    constexpr int kTile = S::kTile, kM = S::kM, kD = S::kD, kN = S::kN, kHeads = S::kHeads, kWarps = S::kWarps, kStages = S::kStages, kRow = S::kRow, kPiece = S::kPiece;
     extern __shared__ __align__(1024) unsigned char ring[];
     __shared__ Piece s_piece[2 * kWarps];
     // (read two heads at a time)
@@ -205,11 +214,12 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
     __shared__ int s_entry[2 * kWarps];                                          // the pieces that there are, in the order of the list
     __shared__ int s_last[2], s_cta0[2], s_ctas[2];                              // segments that other CTAs have pieces of; which CTAs
 
+    auto tiles_of = [](int len) { return tiles_in<kTile>(len); };
     pdl_launch_dependents();
     pdl_wait();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int segments = a.c.kv_heads * parts;                                   // per sequence
-    const int64_t most64 = a.max_pages * a.c.block_size, most = most64 < 0x7fffffff ? most64 : 0x7fffffff;
+    const int64_t most64 = a.max_pages * a.c.block_size, most = most64 < 0x7fffff00 ? most64 : 0x7fffff00;
 
     // ---- shares: every warp for itself, a lane for a stretch of sequences -------------------------------------------
     const int stretch = (a.batch + 31) >> 5, lane_b = lane * stretch;
@@ -245,7 +255,7 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
     unsigned char* const my_ring = ring + warp * (kStages * S::kStageBytes);
     const uint32_t my_ring_at = smem_addr(my_ring);
     const int row_bytes = a.c.dim * (kE4m3 ? 1 : 2);
-    const bool paged16 = a.c.block_size % kTile == 0;
+    const bool paged16 = a.c.block_size % kBlock == 0;
     const int g = lane >> 2, t4 = lane & 3;
     if (row_bytes < kRow) {                                         // channels behind head_dim: zeros once, they are never copied to
         for (int i = lane * 16; i < kStages * S::kStageBytes; i += 512) *reinterpret_cast<uint4*>(my_ring + i) = {0, 0, 0, 0};
@@ -317,21 +327,23 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
     const int copy_row = lane / S::kWords, word = lane % S::kWords;
     auto swizzle = [](int r, int w) { return S::kWords >= 8 ? (w & ~7) | ((w ^ r) & 7) : (w ^ (r >> 1)) & 3; };
     const uint32_t copy_dst = copy_row * kRow + swizzle(copy_row, word) * 16;
+    const unsigned page_limit = a.c.num_blocks < 0x7fffffff ? (unsigned)a.c.num_blocks : 0x7fffffffu;
     const bool word_there = word * 16 < row_bytes, dense = a.c.st == kRow;
     const int64_t lane_from = copy_row * a.c.st + word * 16, v_less_k = a.c.v - a.c.k;
     const float* const lane_scale = kE4m3 ? (lane < 16 ? a.c.k_scale : a.c.v_scale) + (lane & 15) * a.c.sst : nullptr;
-    auto copy_tile = [&](int stage) {
-        const uint32_t ks = my_ring_at + stage * S::kStageBytes, vs = ks + kTile * kRow;
-        const int head = in.head, rows = in.len - in.t * kTile;                   // rows that exist: at least 16, but at a sequence's end
+    auto copy_block = [&](uint32_t ks, uint32_t vs, uint32_t scales, int token0) {
+        const int rows = in.len - token0;                                         // that exist: at least 16, but at a sequence's end
         auto dst_of = [&](int j) { return j * S::kRowsPerCopy * kRow + (copy_dst ^ (S::kWords >= 8 ? ((j * S::kRowsPerCopy) & 7) * 16 : 0)); };
         if (paged16) {
             if ((unsigned)(page_at - page_base) >= 32u) {
                 page_base = page_at;
                 pages = table_entry(in.b, in.len, page_base + lane);
             }
-            const int64_t p = __shfl_sync(0xffffffffu, pages, page_at - page_base);
-            if (rows >= kTile && p >= 0 && p < a.c.num_blocks) {                  // a whole tile of a page
-                const unsigned char* k_row = a.c.k + p * a.c.sb + page_off * a.c.st + head * a.c.sh + lane_from;
+            const int page = __shfl_sync(0xffffffffu, pages, page_at - page_base), off = page_off;
+            page_off += kBlock;
+            if (page_off == a.c.block_size) { page_off = 0; ++page_at; }
+            if (rows >= kBlock && (unsigned)page < page_limit) {                  // a whole block of a page
+                const unsigned char* k_row = a.c.k + page * a.c.sb + off * a.c.st + in.head * a.c.sh + lane_from;
                 const unsigned char* v_row = k_row + v_less_k;
                 if (word_there) {
                     if (dense) {
@@ -350,14 +362,12 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
                         }
                     }
                 }
-                if (kE4m3) copy4(vs + kTile * kRow + lane * 4, lane_scale + p * a.c.ssb + page_off * a.c.sst + head * a.c.ssh, true);
-                page_off += kTile;
-                if (page_off == a.c.block_size) { page_off = 0; ++page_at; }
+                if (kE4m3) copy4(scales + lane * 4, lane_scale + page * a.c.ssb + off * a.c.sst + in.head * a.c.ssh, true);
                 return;
             }
         }
         // a sequence's end, rows with pages of their own, pages that do not exist: row by row, zeros where there is none
-        const int r16 = lane & 15, token = in.t * kTile + r16;
+        const int r16 = lane & 15, token = token0 + r16;
         bool there = r16 < rows;
         int64_t p = 0, off = 0;
         if (there) {
@@ -369,7 +379,7 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
                 report_status(a.status, kDevBadPage);
             }
         }
-        const long long row_from = there ? p * a.c.sb + off * a.c.st + head * a.c.sh : -1;
+        const long long row_from = there ? p * a.c.sb + off * a.c.st + in.head * a.c.sh : -1;
 #pragma unroll 1
         for (int j = 0; j < S::kCopies; ++j) {
             const long long from = __shfl_sync(0xffffffffu, row_from, copy_row + j * S::kRowsPerCopy);
@@ -379,34 +389,53 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
             copy16(vs + dst_of(j), ok ? row + v_less_k : a.c.v, ok);
         }
         if (kE4m3) {
-            const float* s = (lane < 16 ? a.c.k_scale : a.c.v_scale) + (there ? p * a.c.ssb + off * a.c.sst + head * a.c.ssh : 0);
-            copy4(vs + kTile * kRow + lane * 4, s, there);
-        }
-        if (paged16) {
-            page_off += kTile;
-            if (page_off == a.c.block_size) { page_off = 0; ++page_at; }
+            const float* s = (lane < 16 ? a.c.k_scale : a.c.v_scale) + (there ? p * a.c.ssb + off * a.c.sst + in.head * a.c.ssh : 0);
+            copy4(scales + lane * 4, s, there);
         }
     };
-    auto next_tile = [&] {
+    auto copy_tile = [&](int stage) {
+        const uint32_t ks = my_ring_at + stage * S::kStageBytes;
+#pragma unroll
+        for (int h = 0; h < kM; ++h)
+            copy_block(ks + h * kBlock * kRow, ks + (kTile + h * kBlock) * kRow, ks + 2 * kTile * kRow + h * 2 * kBlock * 4, in.t * kTile + h * kBlock);
+    };
+    // The queries of `in`'s segment on their way to L1 when its first tile is copied: asked for when they are needed, they would queue
+    // behind all the tiles that the SM's warps have asked for before.
+    auto queries_ahead = [&] {
+        constexpr int kLines = kD * 2 / 128 > 0 ? kD * 2 / 128 : 1;               // of a row
+        for (int x = lane; x < kHeads * kLines; x += 32) {
+            const int col = x / kLines;
+            if (in.part * kHeads + col < group)
+                prefetch_l1(a.q + (int64_t)in.b * a.q_row + (int64_t)(in.head * group + in.part * kHeads + col) * a.q_head + x % kLines * 64);
+        }
+    };
+    auto next_tile = [&](bool more) {
         if (++in.t < in.tiles) return;
         in.t = 0;
         page_at = page_off = 0;
-        if (next_segment(in)) return;
+        if (next_segment(in)) {
+            if (more) queries_ahead();
+            return;
+        }
         if (next_b != in.b) look_at(in.b);
         in.len = next_len;
         in.tiles = tiles_of(in.len);
         pages = next_pages;
         page_base = 0;
+        if (more) queries_ahead();
         look_at(in.b + 1);
     };
 
     const Result result(a);
     uint32_t q[kD / 16][kN][2];
     float o[kD / 16][kN][4], m[kN][2], l[kN][2], to_score[kN][2];
+    float v_most = 0.f, v_up = 0.f;                                                // ... the largest scale that goes with it, and what they are multiplied by
     int value_exp = 15;                                                            // exponent field that the values' scales are relative to
     auto begin_segment = [&] {
         const int head0 = at.head * group + at.part * kHeads, heads = min(kHeads, group - at.part * kHeads);
         value_exp = 15;
+        v_most = 0.f;
+        v_up = __uint_as_float(245u << 23);
 #pragma unroll
         for (int n = 0; n < kN; ++n) {
             const __nv_bfloat16* row = a.q + (int64_t)at.b * a.q_row + (int64_t)(head0 + n * 8 + g) * a.q_head;
@@ -463,70 +492,106 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
     const int mi = lane >> 3, lr = lane & 7, k_r = lr + (mi & 1) * 8, v_r = kE4m3 ? k_r : lr + (mi >> 1) * 8;
     const uint32_t k_lane = k_r * kRow + swizzle(k_r, mi >> 1) * 16, v_lane = v_r * kRow + swizzle(v_r, kE4m3 ? mi >> 1 : mi & 1) * 16;
     auto words_on = [](uint32_t lane_at, int w) { return (lane_at ^ ((w & 7) * 16)) + (w & ~7) * 16; };
+    constexpr int kLoads = kD / (kE4m3 ? 32 : 16);                                 // of a block's keys (or values)
+    constexpr bool kEarly = kM * kLoads <= 8;                                      // values to registers in front of the softmax
     auto work_on = [&](int stage) {
         const uint32_t ks = my_ring_at + stage * S::kStageBytes, k_at = ks + k_lane, v_at = ks + kTile * kRow + v_lane;
-        float s[kN][4];
+        auto load_keys = [&](uint32_t (&f)[4], int h, int x) { ldmatrix4(f, words_on(k_at, 2 * x) + h * kBlock * kRow); };
+        auto load_values = [&](uint32_t (&f)[4], int h, int x) { ldmatrix4_trans(f, words_on(v_at, 2 * x) + h * kBlock * kRow); };
+        // scores: rows of the A operand are tokens; two sums each, so that they do not wait for one another
+        float s[kM][kN][4], s2[kM][kN][4];
 #pragma unroll
-        for (int n = 0; n < kN; ++n)
+        for (int h = 0; h < kM; ++h)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s[n][i] = 0.f;
-        // scores: rows of the A operand are tokens
-        {
+            for (int n = 0; n < kN; ++n)
 #pragma unroll
-            for (int c = 0; c < kD / 16; c += kE4m3 ? 2 : 1) {
-                uint32_t f[4];
-                ldmatrix4(f, words_on(k_at, kE4m3 ? c : 2 * c));
-                if (kE4m3) {
+                for (int i = 0; i < 4; ++i) s[h][n][i] = s2[h][n][i] = 0.f;
+        constexpr int kAhead = kLoads < 8 / kM ? kLoads : 8 / kM;
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const uint32_t x = f[2 * h], y = f[2 * h + 1];
-                        const uint32_t a0 = cvt_e4m3x2_to_f16x2((uint16_t)x), a2 = cvt_e4m3x2_to_f16x2((uint16_t)(x >> 16));
-                        const uint32_t a1 = cvt_e4m3x2_to_f16x2((uint16_t)y), a3 = cvt_e4m3x2_to_f16x2((uint16_t)(y >> 16));
+        for (int x0 = 0; x0 < kLoads; x0 += kAhead) {
+            uint32_t f[kM][kAhead][4];
 #pragma unroll
-                        for (int n = 0; n < kN; ++n) mma<true>(s[n], a0, a1, a2, a3, q[c + h][n][0], q[c + h][n][1]);
+            for (int x = 0; x < kAhead; ++x)
+#pragma unroll
+                for (int h = 0; h < kM; ++h) load_keys(f[h][x], h, x0 + x);
+#pragma unroll
+            for (int x = 0; x < kAhead; ++x)
+#pragma unroll
+                for (int h = 0; h < kM; ++h) {
+                    const uint32_t* y = f[h][x];
+                    if (kE4m3) {
+                        uint32_t lo[4], hi[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) widen(y[i], lo[i], hi[i]);
+#pragma unroll
+                        for (int n = 0; n < kN; ++n) {
+                            const int c = 2 * (x0 + x);
+                            mma<true>(s[h][n], lo[0], lo[1], hi[0], hi[1], q[c][n][0], q[c][n][1]);
+                            mma<true>(s2[h][n], lo[2], lo[3], hi[2], hi[3], q[c + 1][n][0], q[c + 1][n][1]);
+                        }
+                    } else {
+#pragma unroll
+                        for (int n = 0; n < kN; ++n) mma<false>((x & 1) ? s2[h][n] : s[h][n], y[0], y[1], y[2], y[3], q[x0 + x][n][0], q[x0 + x][n][1]);
                     }
-                } else {
-#pragma unroll
-                    for (int n = 0; n < kN; ++n) mma<false>(s[n], f[0], f[1], f[2], f[3], q[c][n][0], q[c][n][1]);
                 }
-            }
         }
-        float k_scale[2], v_scale[2];                                              // of tokens g and g + 8
+        uint32_t vf[kM][kEarly ? kLoads : 1][4];
+        if (kEarly) {
+#pragma unroll
+            for (int x = 0; x < kLoads; ++x)
+#pragma unroll
+                for (int h = 0; h < kM; ++h) load_values(vf[h][x], h, x);
+        }
+        float k_scale[kM][2], v_scale[kM][2];                                      // of tokens g and g + 8
         if (kE4m3) {
             const float* sc = reinterpret_cast<const float*>(my_ring + stage * S::kStageBytes + 2 * kTile * kRow);
 #pragma unroll
-            for (int h = 0; h < 2; ++h) { k_scale[h] = sc[g + 8 * h]; v_scale[h] = sc[kTile + g + 8 * h]; }
+            for (int h = 0; h < kM; ++h)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) { k_scale[h][i] = sc[h * 32 + g + 8 * i]; v_scale[h][i] = sc[h * 32 + 16 + g + 8 * i]; }
         }
         const int rows = at.len - at.t * kTile;
+#pragma unroll
+        for (int h = 0; h < kM; ++h)
+#pragma unroll
+            for (int n = 0; n < kN; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[h][n][i] = (s[h][n][i] + s2[h][n][i]) * (kE4m3 ? k_scale[h][i >> 1] * to_score[n][i & 1] : to_score[n][i & 1]);
+        if (rows < kTile) {
+#pragma unroll
+            for (int h = 0; h < kM; ++h)
+#pragma unroll
+                for (int n = 0; n < kN; ++n)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (h * kBlock + g + 8 * (i >> 1) >= rows) s[h][n][i] = -INFINITY;
+        }
         float top[kN][2];
         bool raised = false;
 #pragma unroll
         for (int n = 0; n < kN; ++n)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s[n][i] *= kE4m3 ? k_scale[i >> 1] * to_score[n][i & 1] : to_score[n][i & 1];
-        if (rows < kTile) {
-#pragma unroll
-            for (int n = 0; n < kN; ++n)
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (g + 8 * (i >> 1) >= rows) s[n][i] = -INFINITY;
-        }
-#pragma unroll
-        for (int n = 0; n < kN; ++n)
-#pragma unroll
             for (int i = 0; i < 2; ++i) {
-                top[n][i] = fmaxf(s[n][i], s[n][2 + i]);
+                top[n][i] = fmaxf(s[0][n][i], s[0][n][2 + i]);
+#pragma unroll
+                for (int h = 1; h < kM; ++h) top[n][i] = fmaxf(top[n][i], fmaxf(s[h][n][i], s[h][n][2 + i]));
                 raised |= top[n][i] > m[n][i] + kSlack;
             }
-        int exp_now = value_exp;
+        float v_top = 0.f;
         if (kE4m3) {
-            exp_now = max(value_exp, (int)(__float_as_uint(fmaxf(fabsf(v_scale[0]), fabsf(v_scale[1]))) >> 23));
-            raised |= exp_now != value_exp;
+#pragma unroll
+            for (int h = 0; h < kM; ++h) v_top = fmaxf(v_top, fmaxf(fabsf(v_scale[h][0]), fabsf(v_scale[h][1])));
+            raised |= v_top > v_most;
         }
         if (__any_sync(0xffffffffu, raised)) {
-            if (kE4m3) exp_now = __reduce_max_sync(0xffffffffu, exp_now);
-            const float down = kE4m3 ? exp2_approx((float)(value_exp - exp_now)) : 1.f;
-            value_exp = exp_now;
+            float down = 1.f;
+            if (kE4m3) {                                                           // the next power of two above the largest scale
+                const int e = __reduce_max_sync(0xffffffffu, max(value_exp, (int)(__float_as_uint(v_top) >> 23)));
+                down = exp2_approx((float)(value_exp - e));
+                value_exp = e;
+                v_most = __uint_as_float((uint32_t)e << 23 | 0x7fffffu);
+                v_up = __uint_as_float((uint32_t)(260 - e) << 23);                 // 2^(6 - (e - 127)): weights times scales below 2^15
+            }
 #pragma unroll
             for (int n = 0; n < kN; ++n)
 #pragma unroll
@@ -543,52 +608,55 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
                     for (int c = 0; c < kD / 16; ++c) { o[c][n][i] *= fd; o[c][n][2 + i] *= fd; }
                 }
         }
-        uint32_t hi[kN][2], lo[kN][2];
-        const float up = kE4m3 ? __uint_as_float((uint32_t)(260 - value_exp) << 23) : 1.f;    // 2^(6 - (value_exp - 127)): products below 2^15
-        float v_up[2] = {1.f, 1.f};
-        if (kE4m3) { v_up[0] = v_scale[0] * up; v_up[1] = v_scale[1] * up; }
+        uint32_t hi[kM][kN][2], lo[kM][kN][2];
 #pragma unroll
-        for (int n = 0; n < kN; ++n)
+        for (int h = 0; h < kM; ++h) {
+            float up[2] = {1.f, 1.f};
+            if (kE4m3) { up[0] = v_scale[h][0] * v_up; up[1] = v_scale[h][1] * v_up; }
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                float p[2];
+            for (int n = 0; n < kN; ++n)
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    p[i] = exp2_approx(s[n][2 * h + i] - m[n][i]);
-                    l[n][i] += p[i];
-                    if (kE4m3) p[i] *= v_up[h];
+                for (int r = 0; r < 2; ++r) {
+                    float p[2];
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        p[i] = exp2_approx(s[h][n][2 * r + i] - m[n][i]);
+                        l[n][i] += p[i];
+                        if (kE4m3) p[i] *= up[r];
+                    }
+                    split2<kE4m3>(p[0], p[1], hi[h][n][r], lo[h][n][r]);
+                    hi[h][n][r] = transposed(hi[h][n][r]);
+                    lo[h][n][r] = transposed(lo[h][n][r]);
                 }
-                split2<kE4m3>(p[0], p[1], hi[n][h], lo[n][h]);
-                hi[n][h] = transposed(hi[n][h]);
-                lo[n][h] = transposed(lo[n][h]);
-            }
+        }
         // values: rows of the A operand are channels
 #pragma unroll
-        for (int c = 0; c < kD / 16; c += kE4m3 ? 2 : 1) {
-            uint32_t f[4];
-            if (kE4m3) {
-                // a lane's word holds channels 2g and 2g + 1 of two tokens: the first are row g, the second row g + 8
-                ldmatrix4_trans(f, words_on(v_at, c));
+        for (int x = 0; x < kLoads; ++x)
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const uint32_t x = prmt(f[2 * h], 0x3120), y = prmt(f[2 * h + 1], 0x3120);
-                    const uint32_t a0 = cvt_e4m3x2_to_f16x2((uint16_t)x), a1 = cvt_e4m3x2_to_f16x2((uint16_t)(x >> 16));
-                    const uint32_t a2 = cvt_e4m3x2_to_f16x2((uint16_t)y), a3 = cvt_e4m3x2_to_f16x2((uint16_t)(y >> 16));
+            for (int h = 0; h < kM; ++h) {
+                uint32_t late[4];
+                if (!kEarly) load_values(late, h, x);
+                const uint32_t* y = kEarly ? vf[h][kEarly ? x : 0] : late;
+                if (kE4m3) {
+                    // a lane's word holds channels 2g and 2g + 1 of two tokens: the first are row g, the second row g + 8
+                    uint32_t even[4], odd[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) widen(prmt(y[i], 0x3120), even[i], odd[i]);
 #pragma unroll
                     for (int n = 0; n < kN; ++n) {
-                        mma<true>(o[c + h][n], a0, a1, a2, a3, hi[n][0], hi[n][1]);
-                        mma<true>(o[c + h][n], a0, a1, a2, a3, lo[n][0], lo[n][1]);
+                        mma<true>(o[2 * x][n], even[0], odd[0], even[1], odd[1], hi[h][n][0], hi[h][n][1]);
+                        mma<true>(o[2 * x + 1][n], even[2], odd[2], even[3], odd[3], hi[h][n][0], hi[h][n][1]);
+                        mma<true>(o[2 * x][n], even[0], odd[0], even[1], odd[1], lo[h][n][0], lo[h][n][1]);
+                        mma<true>(o[2 * x + 1][n], even[2], odd[2], even[3], odd[3], lo[h][n][0], lo[h][n][1]);
+                    }
+                } else {
+#pragma unroll
+                    for (int n = 0; n < kN; ++n) {
+                        mma<false>(o[x][n], y[0], y[1], y[2], y[3], hi[h][n][0], hi[h][n][1]);
+                        mma<false>(o[x][n], y[0], y[1], y[2], y[3], lo[h][n][0], lo[h][n][1]);
                     }
                 }
-            } else {
-                ldmatrix4_trans(f, words_on(v_at, 2 * c));
-#pragma unroll
-                for (int n = 0; n < kN; ++n) {
-                    mma<false>(o[c][n], f[0], f[1], f[2], f[3], hi[n][0], hi[n][1]);
-                    mma<false>(o[c][n], f[0], f[1], f[2], f[3], lo[n][0], lo[n][1]);
-                }
             }
-        }
     };
     // A piece's sums, as they lie in the lanes, with their statistics; `last`: the warp's last piece, kept in shared memory, else in scratch.
     auto keep_piece = [&](bool last, float* sums) {
@@ -607,6 +675,7 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
     bool kept = false;
     if (lane < 2) s_piece[2 * warp + lane].tile0 = -1;
     __syncwarp();
+    if (todo > 0) queries_ahead();
     int to = 0, from = 0;                                                          // stages: of the next copy, of the next tile's work
     for (int i = 1 - kStages; i < todo; ++i) {
         if (i >= 0) {
@@ -615,7 +684,7 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
         }
         if (i < todo - (kStages - 1)) {
             copy_tile(to);
-            next_tile();
+            next_tile(i < todo - kStages);
             to = to + 1 == kStages ? 0 : to + 1;
         }
         copies_end();
@@ -866,13 +935,13 @@ template <class F>
 auto with_shape(bool e4m3, int64_t dim, int64_t group, F&& f) {
     const bool wide = group > 8;
     if (e4m3) {
-        if (dim <= 64) return wide ? f(Shape<true, 64, 2, 8, 6>()) : f(Shape<true, 64, 1, 16, 6>());
-        if (dim <= 128) return wide ? f(Shape<true, 128, 2, 8, 6>()) : f(Shape<true, 128, 1, 16, 3>());
-        return f(Shape<true, 256, 1, 8, 3>());
+        if (dim <= 64) return wide ? f(Shape<true, 64, 2, 1, 8, 6>()) : f(Shape<true, 64, 1, 2, 16, 3>());
+        if (dim <= 128) return wide ? f(Shape<true, 128, 2, 1, 8, 6>()) : f(Shape<true, 128, 1, 2, 8, 3>());
+        return f(Shape<true, 256, 1, 1, 8, 3>());
     }
-    if (dim <= 64) return wide ? f(Shape<false, 64, 2, 8, 6>()) : f(Shape<false, 64, 1, 16, 3>());
-    if (dim <= 128) return wide ? f(Shape<false, 128, 2, 8, 3>()) : f(Shape<false, 128, 1, 8, 3>());
-    return f(Shape<false, 256, 1, 4, 3>());
+    if (dim <= 64) return wide ? f(Shape<false, 64, 2, 1, 8, 6>()) : f(Shape<false, 64, 1, 2, 8, 3>());
+    if (dim <= 128) return wide ? f(Shape<false, 128, 2, 1, 8, 3>()) : f(Shape<false, 128, 1, 1, 8, 3>());
+    return f(Shape<false, 256, 1, 1, 4, 3>());
 }
 
 }  // namespace
