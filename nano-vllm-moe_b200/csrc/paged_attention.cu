@@ -6,7 +6,7 @@
 // What bounds it is the cache's bytes: 2 D of them (bf16: 4 D) per token and key head, each read once, against 4 D
 // multiplications for each of the group of query heads that share it.
 //
-// Work.  The cached tokens of a key head are cut into tiles of 16; a query group ("segment": one sequence, one key head, up to
+// Work.  The cached tokens of a key head are cut into tiles of 16 or 32; a query group ("segment": one sequence, one key head, up to
 // 8 or 16 of its query heads) is a run of tiles, and all segments one behind the other are one list.  CTAs (one per SM) take equal
 // shares of the list, their warps equal shares of that, so a batch of any lengths keeps every SM busy to the end, and a
 // captured call follows lengths that change: the shares are computed on the device, by every CTA for itself, from the
@@ -67,7 +67,6 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
 __device__ __forceinline__ void copy4(uint32_t dst, const void* src, bool there) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(there ? 4 : 0) : "memory");
 }
-__device__ __forceinline__ void prefetch_l1(const void* p) { asm volatile("prefetch.global.L1 [%0];" ::"l"(p)); }
 __device__ __forceinline__ void copies_end() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int kLeft>
 __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory"); }
@@ -144,10 +143,8 @@ __device__ __forceinline__ int arrive(int* counter) {
 }
 
 // Tiles of a sequence; an empty one has one as well, of nothing, so that its zeros are written like any result.
-__device__ __forceinline__ int tokens_of(const AttnArgs& a, int64_t b, int64_t most) {
-    const int len = ld_dep(a.lens + b);
-    return len < 0 ? 0 : (int64_t)len > most ? (int)most : len;
-}
+__device__ __forceinline__ int within(int len, int64_t most) { return len < 0 ? 0 : (int64_t)len > most ? (int)most : len; }
+__device__ __forceinline__ int tokens_of(const AttnArgs& a, int64_t b, int64_t most) { return within(ld_dep(a.lens + b), most); }
 template <int kTile>
 __device__ __forceinline__ int tiles_in(int len) { return len > kTile ? (int)(((unsigned)len + kTile - 1) / kTile) : 1; }
 
@@ -155,10 +152,6 @@ __device__ __forceinline__ int tiles_in(int len) { return len > kTile ? (int)(((
 __device__ __forceinline__ int64_t quotient(int64_t n, int64_t d) {
     return ((n | d) >> 32) == 0 ? (int64_t)((uint32_t)n / (uint32_t)d) : n / d;
 }
-// Whose share of `total` tiles among `parts` a tile is in: part p has [total p / parts, total (p + 1) / parts).
-__device__ __forceinline__ int64_t share_begin(int64_t total, int parts, int64_t p) { return quotient(total * p, parts); }
-__device__ __forceinline__ int share_of(int64_t total, int parts, int64_t tile) { return (int)quotient((tile + 1) * parts - 1, total); }
-
 struct Piece {                  // part of a segment
     int64_t tile0;              // the segment's first tile in the list, -1: none
     int tiles, b, head0, heads; // its tiles, sequence and query heads
@@ -224,14 +217,16 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
     // ---- shares: every warp for itself, a lane for a stretch of sequences -------------------------------------------
     const int stretch = (a.batch + 31) >> 5, lane_b = lane * stretch;
     int64_t mine = 0;
-    int lane_len = 0;                                                             // of the stretch's last
+    int lane_len = 0, lane_most = 0;                                              // of the stretch's last; most tiles
 #pragma unroll 8
     for (int i = 0; i < stretch; ++i) {
         if (lane_b + i < a.batch) {
             const int len = ld_dep(a.lens + lane_b + i);
             if (len > most && blockIdx.x == 0) report_status(a.status, kDevBadPage);
             lane_len = len < 0 ? 0 : len < most ? len : (int)most;
-            mine += tiles_of(lane_len);
+            const int tiles = tiles_of(lane_len);
+            mine += tiles;
+            lane_most = tiles > lane_most ? tiles : lane_most;
         }
     }
     mine *= segments;
@@ -243,13 +238,72 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
     }
     const int64_t total = __shfl_sync(0xffffffffu, before, 31);
     before -= mine;
-    // one tile per warp at least
-    const int64_t wanted = (total + kWarps - 1) / kWarps;
-    const int ctas = wanted < gridDim.x ? (int)wanted : (int)gridDim.x;
-    if ((int)blockIdx.x >= ctas) return;
-    const int64_t cta0 = share_begin(total, ctas, blockIdx.x), cta1 = share_begin(total, ctas, blockIdx.x + 1);
-    const int64_t begin = cta0 + (cta1 - cta0) * warp / kWarps, todo64 = cta0 + (cta1 - cta0) * (warp + 1) / kWarps - begin;
-    const int todo = (int)(todo64 < 0x7fffffff ? todo64 : 0x7fffffff);
+    const int longest = __reduce_max_sync(0xffffffffu, lane_most);
+    int64_t share = quotient(total + gridDim.x - 1, gridDim.x);                   // of a CTA; a tile per warp at least
+    if (share < kWarps) share = kWarps;
+    // Where a tile of the list is: its sequence, the place in it, the sequence's length.
+    struct Found { int b, len; int64_t inside; };
+    auto find = [&](int64_t tile) {
+        Found f;
+        f.inside = tile - before;
+        const int where = __ffs(__ballot_sync(0xffffffffu, f.inside >= 0 && f.inside < mine)) - 1;
+        f.inside = __shfl_sync(0xffffffffu, f.inside, where);
+        f.b = where;
+        f.len = __shfl_sync(0xffffffffu, lane_len, where);
+        if (stretch > 1) for (int b0 = where * stretch;; b0 += 32) {              // (it is one of the stretch's)
+            const int len = b0 + lane < a.batch ? tokens_of(a, b0 + lane, most) : 0;
+            const int64_t all = b0 + lane < a.batch ? (int64_t)tiles_of(len) * segments : 0;
+            int64_t upto = all;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int64_t y = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += y;
+            }
+            const uint32_t beyond = __ballot_sync(0xffffffffu, upto > f.inside);
+            if (beyond) {
+                const int w = __ffs(beyond) - 1;
+                f.b = b0 + w;
+                f.len = __shfl_sync(0xffffffffu, len, w);
+                f.inside -= __shfl_sync(0xffffffffu, upto - all, w);
+                break;
+            }
+            f.inside -= __shfl_sync(0xffffffffu, upto, 31);
+        }
+        return f;
+    };
+    // Joining a segment over CTAs costs as much as some eight tiles per warp.  So where there is a CTA for every segment and none is so much longer
+    // than an even share, each has one; and where the segments are short, shares begin and end with segments.
+    const bool own_cta = a.batch <= gridDim.x && (int64_t)a.batch * segments <= gridDim.x && longest <= share + 8 * kWarps;
+    const bool whole = !own_cta && longest <= 2 * kWarps;
+    int64_t cta0, cta1;
+    Found mid;                                                                    // own_cta: the CTA's segment
+    int mid_segment = 0;
+    if (own_cta) {
+        if ((int)blockIdx.x >= a.batch * segments) return;
+        mid.b = blockIdx.x / segments;
+        mid_segment = blockIdx.x - mid.b * segments;
+        mid.len = tokens_of(a, mid.b, most);
+        cta0 = 0;
+        cta1 = tiles_of(mid.len);
+    } else {
+        cta0 = blockIdx.x * share;
+        cta1 = cta0 + share < total ? cta0 + share : total;
+        if (cta0 >= total) return;
+        if (whole) {
+            auto rounded = [&](int64_t tile) {                                    // to the nearer end of its segment
+                if (tile >= total) return total;
+                const Found f = find(tile);
+                const int tiles = tiles_of(f.len), in_segment = (int)(f.inside - quotient(f.inside, tiles) * tiles);
+                return tile + (2 * in_segment < tiles ? -in_segment : tiles - in_segment);
+            };
+            cta0 = rounded(cta0);
+            cta1 = rounded(cta1);
+            if (cta0 >= cta1) return;
+        }
+    }
+    const int64_t warp_share = (cta1 - cta0 + kWarps - 1) / kWarps, begin = cta0 + warp * warp_share;
+    const int64_t todo64 = cta1 - begin < warp_share ? cta1 - begin : warp_share;
+    const int todo = todo64 < 0 ? 0 : (int)(todo64 < 0x7fffffff ? todo64 : 0x7fffffff);
 
     // ---- a warp's tiles -----------------------------------------------------------------------------------------------
     unsigned char* const my_ring = ring + warp * (kStages * S::kStageBytes);
@@ -273,55 +327,40 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
         ++x.b;
         return false;
     };
-    // Pages of `in` where they hold whole tiles: 32 entries of its table at a time, a lane each, from page_base on
-    int pages = 0, page_base = 0, page_at = 0, page_off = 0;
-    int next_b = -1, next_len = 0, next_pages = 0;                  // the sequence behind it, once it was looked at
-    auto table_entry = [&](int b, int len, int i) {
-        return (int64_t)i * a.c.block_size < len ? ld_dep(a.tables + (int64_t)b * a.ld_tables + i) : 0;
-    };
+    // Nothing that the loop needs is waited for in it: a load queues behind all the copies that the SM's warps have asked for, some 2.5 us.  So lengths and
+    // queries are asked for a segment early, and pages (where they hold whole blocks) come 32 table entries at a time, a lane each, also early: those from
+    // page_base on, the 32 behind them, a sequence's first for its next head, and the next sequence's.
+    int pages = 0, pages_behind = 0, pages_first = 0, page_base = 0, page_at = 0, page_off = 0;
+    int next_len = 0, next_pages = 0, after_len = 0;                // of the sequences behind in.b, behind at.b
+    auto entry = [&](int b, int64_t i) { return paged16 && i < a.max_pages ? ld_dep(a.tables + (int64_t)b * a.ld_tables + i) : -1; };
     auto look_at = [&](int b) {
-        next_b = b;
         if (b < a.batch) {
-            next_len = tokens_of(a, b, most);
-            if (paged16) next_pages = table_entry(b, next_len, lane);
+            next_len = ld_dep(a.lens + b);
+            next_pages = entry(b, lane);
         }
     };
     if (todo > 0) {
-        int64_t inside = begin - before;
-        const int where = __ffs(__ballot_sync(0xffffffffu, inside >= 0 && inside < mine)) - 1;
-        inside = __shfl_sync(0xffffffffu, inside, where);
-        in.b = where;
-        in.len = __shfl_sync(0xffffffffu, lane_len, where);
-        if (stretch > 1) for (int b0 = where * stretch;; b0 += 32) {              // (it is one of the stretch's)
-            const int len = b0 + lane < a.batch ? tokens_of(a, b0 + lane, most) : 0;
-            const int64_t all = b0 + lane < a.batch ? (int64_t)tiles_of(len) * segments : 0;
-            int64_t upto = all;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int64_t y = __shfl_up_sync(0xffffffffu, upto, o);
-                if (lane >= o) upto += y;
-            }
-            const uint32_t beyond = __ballot_sync(0xffffffffu, upto > inside);
-            if (beyond) {
-                const int w = __ffs(beyond) - 1;
-                in.b = b0 + w;
-                in.len = __shfl_sync(0xffffffffu, len, w);
-                inside -= __shfl_sync(0xffffffffu, upto - all, w);
-                break;
-            }
-            inside -= __shfl_sync(0xffffffffu, upto, 31);
-        }
+        Found f = mid;
+        int segment = mid_segment;
+        f.inside = begin;
+        if (!own_cta) f = find(begin);
+        in.b = f.b;
+        in.len = f.len;
         in.tiles = tiles_of(in.len);
-        const int segment = (int)quotient(inside, in.tiles);
-        in.t = (int)(inside - (int64_t)segment * in.tiles);
+        if (!own_cta) segment = (int)quotient(f.inside, in.tiles);
+        in.t = (int)(own_cta ? begin : f.inside - (int64_t)segment * in.tiles);
         in.head = parts == 1 ? segment : segment / parts;
         in.part = segment - in.head * parts;
         at = in;
         if (paged16) {
             page_base = page_at = in.t * kTile / a.c.block_size;
             page_off = in.t * kTile - page_at * a.c.block_size;
-            pages = table_entry(in.b, in.len, page_base + lane);
+            pages = entry(in.b, page_base + lane);
+            pages_behind = entry(in.b, page_base + 32 + lane);
+            pages_first = entry(in.b, lane);
         }
+        look_at(in.b + 1);
+        if (at.b + 1 < a.batch) after_len = ld_dep(a.lens + at.b + 1);
     }
     // copies: lane -> word `word` of the rows copy_row + j * kRowsPerCopy
     const int copy_row = lane / S::kWords, word = lane % S::kWords;
@@ -334,16 +373,19 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
     auto copy_block = [&](uint32_t ks, uint32_t vs, uint32_t scales, int token0) {
         const int rows = in.len - token0;                                         // that exist: at least 16, but at a sequence's end
         auto dst_of = [&](int j) { return j * S::kRowsPerCopy * kRow + (copy_dst ^ (S::kWords >= 8 ? ((j * S::kRowsPerCopy) & 7) * 16 : 0)); };
+        int page = -1, off16 = 0;
         if (paged16) {
-            if ((unsigned)(page_at - page_base) >= 32u) {
+            if (page_at - page_base == 32) {
                 page_base = page_at;
-                pages = table_entry(in.b, in.len, page_base + lane);
+                pages = pages_behind;
+                pages_behind = entry(in.b, page_base + 32 + lane);
             }
-            const int page = __shfl_sync(0xffffffffu, pages, page_at - page_base), off = page_off;
+            page = __shfl_sync(0xffffffffu, pages, page_at - page_base);
+            off16 = page_off;
             page_off += kBlock;
             if (page_off == a.c.block_size) { page_off = 0; ++page_at; }
             if (rows >= kBlock && (unsigned)page < page_limit) {                  // a whole block of a page
-                const unsigned char* k_row = a.c.k + page * a.c.sb + off * a.c.st + in.head * a.c.sh + lane_from;
+                const unsigned char* k_row = a.c.k + page * a.c.sb + off16 * a.c.st + in.head * a.c.sh + lane_from;
                 const unsigned char* v_row = k_row + v_less_k;
                 if (word_there) {
                     if (dense) {
@@ -362,7 +404,7 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
                         }
                     }
                 }
-                if (kE4m3) copy4(scales + lane * 4, lane_scale + page * a.c.ssb + off * a.c.sst + in.head * a.c.ssh, true);
+                if (kE4m3) copy4(scales + lane * 4, lane_scale + page * a.c.ssb + off16 * a.c.sst + in.head * a.c.ssh, true);
                 return;
             }
         }
@@ -371,9 +413,14 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
         bool there = r16 < rows;
         int64_t p = 0, off = 0;
         if (there) {
-            const int i = token / a.c.block_size;
-            off = token - (int64_t)i * a.c.block_size;
-            p = ld_dep(a.tables + (int64_t)in.b * a.ld_tables + i);
+            if (paged16) {
+                p = page;
+                off = off16 + r16;
+            } else {
+                const int i = token / a.c.block_size;
+                off = token - (int64_t)i * a.c.block_size;
+                p = ld_dep(a.tables + (int64_t)in.b * a.ld_tables + i);
+            }
             if (p < 0 || p >= a.c.num_blocks) {
                 there = false;
                 report_status(a.status, kDevBadPage);
@@ -399,30 +446,23 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
         for (int h = 0; h < kM; ++h)
             copy_block(ks + h * kBlock * kRow, ks + (kTile + h * kBlock) * kRow, ks + 2 * kTile * kRow + h * 2 * kBlock * 4, in.t * kTile + h * kBlock);
     };
-    // The queries of `in`'s segment on their way to L1 when its first tile is copied: asked for when they are needed, they would queue
-    // behind all the tiles that the SM's warps have asked for before.
-    auto queries_ahead = [&] {
-        constexpr int kLines = kD * 2 / 128 > 0 ? kD * 2 / 128 : 1;               // of a row
-        for (int x = lane; x < kHeads * kLines; x += 32) {
-            const int col = x / kLines;
-            if (in.part * kHeads + col < group)
-                prefetch_l1(a.q + (int64_t)in.b * a.q_row + (int64_t)(in.head * group + in.part * kHeads + col) * a.q_head + x % kLines * 64);
-        }
-    };
-    auto next_tile = [&](bool more) {
+    auto next_tile = [&] {
         if (++in.t < in.tiles) return;
         in.t = 0;
         page_at = page_off = 0;
         if (next_segment(in)) {
-            if (more) queries_ahead();
+            if (page_base != 0) {
+                page_base = 0;
+                pages = pages_first;
+                pages_behind = entry(in.b, 32 + lane);
+            }
             return;
         }
-        if (next_b != in.b) look_at(in.b);
-        in.len = next_len;
+        in.len = within(next_len, most);
         in.tiles = tiles_of(in.len);
-        pages = next_pages;
         page_base = 0;
-        if (more) queries_ahead();
+        pages = pages_first = next_pages;
+        pages_behind = entry(in.b, 32 + lane);
         look_at(in.b + 1);
     };
 
@@ -431,36 +471,54 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
     float o[kD / 16][kN][4], m[kN][2], l[kN][2], to_score[kN][2];
     float v_most = 0.f, v_up = 0.f;                                                // ... the largest scale that goes with it, and what they are multiplied by
     int value_exp = 15;                                                            // exponent field that the values' scales are relative to
-    auto begin_segment = [&] {
-        const int head0 = at.head * group + at.part * kHeads, heads = min(kHeads, group - at.part * kHeads);
-        value_exp = 15;
-        v_most = 0.f;
-        v_up = __uint_as_float(245u << 23);
+    // Queries are asked for one segment early where registers allow: they queue behind the tiles that the SM's warps have asked for.
+    constexpr bool kQueriesEarly = kN == 1 && kD <= 128;
+    uint32_t q_next[kQueriesEarly ? kD / 16 : 1][kN][2];
+    auto load_queries = [&](uint32_t (&to)[kD / 16][kN][2], const Place& x) {
+        const int head0 = x.head * group + x.part * kHeads, heads = group - x.part * kHeads;
 #pragma unroll
         for (int n = 0; n < kN; ++n) {
-            const __nv_bfloat16* row = a.q + (int64_t)at.b * a.q_row + (int64_t)(head0 + n * 8 + g) * a.q_head;
+            const __nv_bfloat16* row = a.q + (int64_t)x.b * a.q_row + (int64_t)(head0 + n * 8 + g) * a.q_head;
             const bool real = n * 8 + g < heads;
-            uint32_t top = 0;
 #pragma unroll
             for (int s = 0; s < kD / 16; ++s) {
-                uint32_t x = 0, y = 0;
+                to[s][n][0] = to[s][n][1] = 0;
                 if (real && s * 16 < a.c.dim) {
                     if (kE4m3) {
                         const long long w = ld_dep(reinterpret_cast<const long long*>(row + s * 16 + t4 * 4));
-                        x = (uint32_t)w;
-                        y = (uint32_t)(w >> 32);
+                        to[s][n][0] = (uint32_t)w;
+                        to[s][n][1] = (uint32_t)(w >> 32);
                     } else {
-                        x = ld_dep(reinterpret_cast<const int*>(row + s * 16 + t4 * 2));
-                        y = ld_dep(reinterpret_cast<const int*>(row + s * 16 + 8 + t4 * 2));
+                        to[s][n][0] = ld_dep(reinterpret_cast<const int*>(row + s * 16 + t4 * 2));
+                        to[s][n][1] = ld_dep(reinterpret_cast<const int*>(row + s * 16 + 8 + t4 * 2));
                     }
                 }
-                q[s][n][0] = x;
-                q[s][n][1] = y;
-                if (kE4m3) top = __vmaxu2(top, __vmaxu2(x & 0x7fff7fffu, y & 0x7fff7fffu));
             }
+        }
+    };
+    auto begin_segment = [&](bool first) {
+        value_exp = 15;
+        v_most = 0.f;
+        v_up = __uint_as_float(245u << 23);
+        if constexpr (kQueriesEarly) {
+            if (first) load_queries(q_next, at);
+#pragma unroll
+            for (int s = 0; s < kD / 16; ++s)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) q[s][0][i] = q_next[s][0][i];
+            Place next = at;
+            if (next_segment(next) || next.b < a.batch) load_queries(q_next, next);
+        } else {
+            load_queries(q, at);
+        }
+#pragma unroll
+        for (int n = 0; n < kN; ++n) {
             const float base = a.scale * kLog2e;
             if (kE4m3) {
                 // the largest channel to 2^14 .. 2^15: f16 holds those down to 2^-29 of it with all of bf16's bits
+                uint32_t top = 0;
+#pragma unroll
+                for (int s = 0; s < kD / 16; ++s) top = __vmaxu2(top, __vmaxu2(q[s][n][0] & 0x7fff7fffu, q[s][n][1] & 0x7fff7fffu));
                 top = max(top & 0xffffu, top >> 16);
                 top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
                 top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
@@ -675,7 +733,6 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
     bool kept = false;
     if (lane < 2) s_piece[2 * warp + lane].tile0 = -1;
     __syncwarp();
-    if (todo > 0) queries_ahead();
     int to = 0, from = 0;                                                          // stages: of the next copy, of the next tile's work
     for (int i = 1 - kStages; i < todo; ++i) {
         if (i >= 0) {
@@ -684,15 +741,12 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
         }
         if (i < todo - (kStages - 1)) {
             copy_tile(to);
-            next_tile(i < todo - kStages);
+            next_tile();
             to = to + 1 == kStages ? 0 : to + 1;
         }
         copies_end();
         if (i < 0) {
-            if (i == -1 && todo > 0) {
-                begin_segment();
-                if (next_b < 0) look_at(in.b + 1);
-            }
+            if (i == -1 && todo > 0) begin_segment(true);
             continue;
         }
         work_on(from);
@@ -730,10 +784,11 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
         if (++at.t == at.tiles) {
             at.t = 0;
             if (!next_segment(at) && i + 1 < todo) {
-                at.len = tokens_of(a, at.b, most);
+                at.len = within(after_len, most);
                 at.tiles = tiles_of(at.len);
+                if (at.b + 1 < a.batch) after_len = ld_dep(a.lens + at.b + 1);
             }
-            if (i + 1 < todo) begin_segment();
+            if (i + 1 < todo) begin_segment(false);
         }
     }
 
@@ -813,7 +868,7 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
         bool last = false;
         if (tid == 0 ? open0 : open1) {
             const Piece p = s_piece[__ffs(tid == 0 ? open0 : open1) - 1];
-            const int c0 = share_of(total, ctas, p.tile0), count = share_of(total, ctas, p.tile0 + p.tiles - 1) - c0 + 1;
+            const int c0 = (int)quotient(p.tile0, share), count = (int)quotient(p.tile0 + p.tiles - 1, share) - c0 + 1;
             s_cta0[tid] = c0;
             s_ctas[tid] = count;
             last = arrive(a.counters + c0) == count - 1;
@@ -828,57 +883,56 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
         const Piece p = s_piece[__ffs(w == 0 ? open0 : open1) - 1];
         const int c0 = s_cta0[w], count = s_ctas[w];
         auto piece_of = [&](int i) { return pieces + ((int64_t)(c0 + i) * 2 + (i == 0)) * kOut; };
-        // kSlices threads share a fragment's pieces; as many pieces as the rings hold are on their way at a time
+        // kSlices threads share a fragment's pieces, kAtOnce of them on their way at a time, the first in front of the weights
         constexpr int kSlices = S::kThreads > kUnits ? S::kThreads / kUnits : 1, kPerThread = kUnits > S::kThreads ? kUnits / S::kThreads : 1;
-        constexpr int kAtOnce = S::kRing / (kPiece * 4);
-        const float4* const shelf = reinterpret_cast<const float4*>(ring);
+        constexpr int kAtOnce = S::kThreads > 256 ? 8 : 16;
         const int slice = tid / kUnits;
         float4 v[kPerThread];
+        uint4 raw[kAtOnce];
+        auto ask = [&](int unit, int i0) {
 #pragma unroll
-        for (int k = 0; k < kPerThread; ++k) v[k] = {0.f, 0.f, 0.f, 0.f};
-        for (int i0 = 0; i0 < count; i0 += kAtOnce) {
-            const int here = count - i0 < kAtOnce ? count - i0 : kAtOnce;
-            for (int x = tid; x < here * kUnits; x += S::kThreads)
-                copy16(smem_addr(shelf + x), reinterpret_cast<const float4*>(piece_of(i0 + x / kUnits)) + x % kUnits);
-            copies_end();
-            if (i0 == 0) {
-                for (int col = warp; col < kHeads; col += kWarps) {                // a warp for a query head, a lane for a few CTAs
-                    float pm[kMaxCtas / 32], pl[kMaxCtas / 32], top = kNone, sum = 0.f;
+            for (int i = 0; i < kAtOnce; ++i)
+                if (i0 + i * kSlices < count) raw[i] = ld_dep_l2(reinterpret_cast<const uint4*>(piece_of(i0 + i * kSlices)) + unit);
+        };
+        ask(tid % kUnits, slice);
+        for (int col = warp; col < kHeads; col += kWarps) {                        // a warp for a query head, a lane for a few CTAs
+            float pm[kMaxCtas / 32], pl[kMaxCtas / 32], top = kNone, sum = 0.f;
 #pragma unroll
-                    for (int i = 0; i < kMaxCtas / 32; ++i) {
-                        pm[i] = kNone;
-                        pl[i] = 0.f;
-                        if (i * 32 + lane < count) {
-                            pm[i] = ld_dep_l2(piece_of(i * 32 + lane) + kPiece + col);
-                            pl[i] = ld_dep_l2(piece_of(i * 32 + lane) + kPiece + kHeads + col);
-                        }
-                    }
-#pragma unroll
-                    for (int i = 0; i < kMaxCtas / 32; ++i) top = fmaxf(top, pm[i]);
-                    for (int x = 16; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-#pragma unroll
-                    for (int i = 0; i < kMaxCtas / 32; ++i) {
-                        const float f = exp2_approx(pm[i] - top);
-                        sum += f * pl[i];
-                        if (i * 32 + lane < count) s_share[i * 32 + lane][col] = f;
-                    }
-                    for (int x = 16; x; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
-                    if (lane == 0) s_inv[col] = reciprocal(sum);
+            for (int i = 0; i < kMaxCtas / 32; ++i) {
+                pm[i] = kNone;
+                pl[i] = 0.f;
+                if (i * 32 + lane < count) {
+                    pm[i] = ld_dep_l2(piece_of(i * 32 + lane) + kPiece + col);
+                    pl[i] = ld_dep_l2(piece_of(i * 32 + lane) + kPiece + kHeads + col);
                 }
             }
-            copies_wait<0>();
-            __syncthreads();
 #pragma unroll
-            for (int k = 0; k < kPerThread; ++k) {
-                const int unit = (tid + k * S::kThreads) % kUnits, col = (unit >> 5) % kN * 8 + 2 * t4;
-#pragma unroll 4
-                for (int i = slice; i < here; i += kSlices) {
-                    const float4 y = shelf[i * kUnits + unit];
-                    const float2 f = *reinterpret_cast<const float2*>(&s_share[i0 + i][col]);
-                    v[k].x += f.x * y.x; v[k].y += f.y * y.y; v[k].z += f.x * y.z; v[k].w += f.y * y.w;
-                }
+            for (int i = 0; i < kMaxCtas / 32; ++i) top = fmaxf(top, pm[i]);
+            top = warp_max(top);
+#pragma unroll
+            for (int i = 0; i < kMaxCtas / 32; ++i) {
+                const float f = exp2_approx(pm[i] - top);
+                sum += f * pl[i];
+                if (i * 32 + lane < count) s_share[i * 32 + lane][col] = f;
             }
-            __syncthreads();
+            for (int x = 16; x; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+            if (lane == 0) s_inv[col] = reciprocal(sum);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < kPerThread; ++k) {
+            const int unit = (tid + k * S::kThreads) % kUnits, col = (unit >> 5) % kN * 8 + 2 * t4;
+            v[k] = {0.f, 0.f, 0.f, 0.f};
+            for (int i0 = slice; i0 < count; i0 += kAtOnce * kSlices) {
+                if (k > 0 || i0 != slice) ask(unit, i0);
+#pragma unroll
+                for (int i = 0; i < kAtOnce; ++i)
+                    if (i0 + i * kSlices < count) {
+                        const float2 f = *reinterpret_cast<const float2*>(&s_share[i0 + i * kSlices][col]);
+                        v[k].x += f.x * __uint_as_float(raw[i].x); v[k].y += f.y * __uint_as_float(raw[i].y);
+                        v[k].z += f.x * __uint_as_float(raw[i].z); v[k].w += f.y * __uint_as_float(raw[i].w);
+                    }
+            }
         }
         if (kSlices > 1) {
             float4* const sums = reinterpret_cast<float4*>(ring);
@@ -900,7 +954,7 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
                                     *reinterpret_cast<const float2*>(&s_inv[n * 8 + 2 * t4]));
             }
         }
-        __syncthreads();                                                           // s_share, s_inv and the rings are free again
+        __syncthreads();                                                           // s_share and s_inv are free again
     }
 }
 
