@@ -96,6 +96,8 @@ __device__ __forceinline__ float exp2_approx(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
+// Places in the list that a segment takes beside its tiles.
+constexpr int kBegin = 1;
 // The reference of no score at all; exp2(kNone - m) is 0 for that of any.
 constexpr float kNone = -3.402823466e38f;
 // Weights are relative to a score that is at most 2^kSlack below the largest: it follows the maximum only where that
@@ -153,7 +155,7 @@ __device__ __forceinline__ int64_t quotient(int64_t n, int64_t d) {
     return ((n | d) >> 32) == 0 ? (int64_t)((uint32_t)n / (uint32_t)d) : n / d;
 }
 struct Piece {                  // part of a segment
-    int64_t tile0;              // the segment's first tile in the list, -1: none
+    int64_t tile0;              // the place of the segment's first tile, -1: none
     int tiles, b, head0, heads; // its tiles, sequence and query heads
 };
 
@@ -229,36 +231,29 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
             lane_most = tiles > lane_most ? tiles : lane_most;
         }
     }
-    mine *= segments;
-    int64_t before = mine;                                                        // inclusive sum
+    // Sequence b's part of the list: a segment's tiles with kBegin places in front of them, what beginning and ending it takes.
+    auto places_of = [&](int len) { return (int64_t)(tiles_of(len) + kBegin) * segments; };
+    auto sum_upto = [&](int64_t x) {                                              // inclusive, over the lanes
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int64_t y = __shfl_up_sync(0xffffffffu, before, o);
-        if (lane >= o) before += y;
-    }
-    const int64_t total = __shfl_sync(0xffffffffu, before, 31);
-    before -= mine;
-    const int longest = __reduce_max_sync(0xffffffffu, lane_most);
-    int64_t share = quotient(total + gridDim.x - 1, gridDim.x);                   // of a CTA; a tile per warp at least
-    if (share < kWarps) share = kWarps;
-    // Where a tile of the list is: its sequence, the place in it, the sequence's length.
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= o) x += y;
+        }
+        return x;
+    };
+    // The sequence whose part of a list `at` is in, the place in it, the sequence's length.  part_of: a sequence's part by its length; this
+    // lane's stretch begins at `before` and has `mine`.
     struct Found { int b, len; int64_t inside; };
-    auto find = [&](int64_t tile) {
+    auto find = [&](auto part_of, int64_t before, int64_t mine, int64_t place) {
         Found f;
-        f.inside = tile - before;
+        f.inside = place - before;
         const int where = __ffs(__ballot_sync(0xffffffffu, f.inside >= 0 && f.inside < mine)) - 1;
         f.inside = __shfl_sync(0xffffffffu, f.inside, where);
         f.b = where;
         f.len = __shfl_sync(0xffffffffu, lane_len, where);
         if (stretch > 1) for (int b0 = where * stretch;; b0 += 32) {              // (it is one of the stretch's)
             const int len = b0 + lane < a.batch ? tokens_of(a, b0 + lane, most) : 0;
-            const int64_t all = b0 + lane < a.batch ? (int64_t)tiles_of(len) * segments : 0;
-            int64_t upto = all;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int64_t y = __shfl_up_sync(0xffffffffu, upto, o);
-                if (lane >= o) upto += y;
-            }
+            const int64_t all = b0 + lane < a.batch ? part_of(len) : 0, upto = sum_upto(all);
             const uint32_t beyond = __ballot_sync(0xffffffffu, upto > f.inside);
             if (beyond) {
                 const int w = __ffs(beyond) - 1;
@@ -271,39 +266,70 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
         }
         return f;
     };
-    // Joining a segment over CTAs costs as much as some eight tiles per warp.  So where there is a CTA for every segment and none is so much longer
-    // than an even share, each has one; and where the segments are short, shares begin and end with segments.
-    const bool own_cta = a.batch <= gridDim.x && (int64_t)a.batch * segments <= gridDim.x && longest <= share + 8 * kWarps;
-    const bool whole = !own_cta && longest <= 2 * kWarps;
-    int64_t cta0, cta1;
-    Found mid;                                                                    // own_cta: the CTA's segment
-    int mid_segment = 0;
-    if (own_cta) {
+    // Three ways to deal the list out.  (1) To CTAs that work on one segment each, some on the same, where no CTA's share grows much by that: joining
+    // the pieces of two segments takes a CTA twice as long.  Joining over CTAs costs as much as some eight tiles per warp, so where there is a CTA for every
+    // segment and none is that much longer than an even share, each has one.  (2) Short segments: in even shares, rounded to whole segments.
+    // (3) In even shares.
+    const int longest = __reduce_max_sync(0xffffffffu, lane_most), grid = (int)gridDim.x;
+    const bool few = a.batch <= grid && a.batch * segments <= grid;
+    bool apart = few && longest <= 9 * kWarps;                                    // (a share is a tile per warp at least)
+    int64_t total = 0, before = 0, share = kWarps, cta0, cta1;                    // this CTA's places: of the list, or (apart) of one segment's part of it
+    Found own = {};                                                               // apart: that segment
+    int own_segment = 0, own_part = 0, own_parts = 1;                             // ... which of its CTAs this is, and of how many
+    if (apart) {
         if ((int)blockIdx.x >= a.batch * segments) return;
-        mid.b = blockIdx.x / segments;
-        mid_segment = blockIdx.x - mid.b * segments;
-        mid.len = tokens_of(a, mid.b, most);
-        cta0 = 0;
-        cta1 = tiles_of(mid.len);
+        own.b = segments == 1 ? blockIdx.x : blockIdx.x / (unsigned)segments;
+        own_segment = blockIdx.x - own.b * segments;
+        own.len = stretch == 1 ? __shfl_sync(0xffffffffu, lane_len, own.b) : tokens_of(a, own.b, most);
+        cta0 = kBegin;
+        cta1 = kBegin + tiles_of(own.len);
     } else {
-        cta0 = blockIdx.x * share;
-        cta1 = cta0 + share < total ? cta0 + share : total;
-        if (cta0 >= total) return;
-        if (whole) {
-            auto rounded = [&](int64_t tile) {                                    // to the nearer end of its segment
-                if (tile >= total) return total;
-                const Found f = find(tile);
-                const int tiles = tiles_of(f.len), in_segment = (int)(f.inside - quotient(f.inside, tiles) * tiles);
-                return tile + (2 * in_segment < tiles ? -in_segment : tiles - in_segment);
-            };
-            cta0 = rounded(cta0);
-            cta1 = rounded(cta1);
-            if (cta0 >= cta1) return;
+        mine = (mine + (int64_t)kBegin * (a.batch - lane_b < 0 ? 0 : a.batch - lane_b < stretch ? a.batch - lane_b : stretch)) * segments;
+        const int64_t before_end = sum_upto(mine);
+        total = __shfl_sync(0xffffffffu, before_end, 31);
+        before = before_end - mine;
+        share = quotient(total + grid - 1, grid);
+        if (share < kWarps) share = kWarps;
+        if (few) {
+            const int64_t cta_share = longest <= share + 8 * kWarps ? longest : share + share / 16;
+            auto units_of = [&](int len) { return quotient(tiles_of(len) + cta_share - 1, cta_share) * segments; };      // CTAs of a sequence
+            int64_t units = 0;
+            if (stretch == 1) units = lane < a.batch ? units_of(lane_len) : 0;
+            else for (int i = 0; i < stretch; ++i)
+                if (lane_b + i < a.batch) units += units_of(tokens_of(a, lane_b + i, most));
+            const int64_t upto = sum_upto(units), all = __shfl_sync(0xffffffffu, upto, 31);
+            apart = all <= grid;
+            if (apart) {
+                if ((int)blockIdx.x >= all) return;
+                own = find(units_of, upto - units, units, blockIdx.x);
+                own_parts = (int)quotient(tiles_of(own.len) + cta_share - 1, cta_share);
+                own_segment = (int)own.inside / own_parts;
+                own_part = (int)own.inside - own_segment * own_parts;
+                cta0 = kBegin + own_part * cta_share;
+                cta1 = kBegin + tiles_of(own.len);
+                if (cta1 > cta0 + cta_share) cta1 = cta0 + cta_share;
+            }
+        }
+        if (!apart) {
+            cta0 = blockIdx.x * share;
+            cta1 = cta0 + share < total ? cta0 + share : total;
+            if (cta0 >= total) return;
+            if (longest <= 2 * kWarps) {
+                auto rounded = [&](int64_t place) {                               // to the nearer end of its segment
+                    if (place >= total) return total;
+                    const Found f = find(places_of, before, mine, place);
+                    const int places = tiles_of(f.len) + kBegin, in_segment = (int)(f.inside - quotient(f.inside, places) * places);
+                    return place + (2 * in_segment < places ? -in_segment : places - in_segment);
+                };
+                cta0 = rounded(cta0);
+                cta1 = rounded(cta1);
+                if (cta0 >= cta1) return;
+            }
         }
     }
     const int64_t warp_share = (cta1 - cta0 + kWarps - 1) / kWarps, begin = cta0 + warp * warp_share;
-    const int64_t todo64 = cta1 - begin < warp_share ? cta1 - begin : warp_share;
-    const int todo = todo64 < 0 ? 0 : (int)(todo64 < 0x7fffffff ? todo64 : 0x7fffffff);
+    const int64_t span64 = cta1 - begin < warp_share ? cta1 - begin : warp_share;
+    const int span = span64 < 0 ? 0 : (int)(span64 < 0x3fffffff ? span64 : 0x3fffffff);                  // this warp's places: from `begin` on
 
     // ---- a warp's tiles -----------------------------------------------------------------------------------------------
     unsigned char* const my_ring = ring + warp * (kStages * S::kStageBytes);
@@ -317,9 +343,10 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
     }
 
     struct Place {
-        int b, head, part, t, len, tiles;                           // sequence, key head, part of its query heads, tile
+        int b, head, part, t, len, tiles, place;                    // sequence, key head, part of its query heads, tile; its place from `begin` on
     } in, at;                                                       // of the next tile to copy, and to work on
     auto next_segment = [&](Place& x) {                             // whether it is one of the same sequence
+        x.place += kBegin;
         if (++x.part < parts) return true;
         x.part = 0;
         if (++x.head < a.c.kv_heads) return true;
@@ -339,16 +366,18 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
             next_pages = entry(b, lane);
         }
     };
-    if (todo > 0) {
-        Found f = mid;
-        int segment = mid_segment;
-        f.inside = begin;
-        if (!own_cta) f = find(begin);
+    in.place = at.place = 0;
+    if (span > 0) {
+        Found f = own;
+        int segment = own_segment;
+        if (!apart) f = find(places_of, before, mine, begin);
         in.b = f.b;
         in.len = f.len;
         in.tiles = tiles_of(in.len);
-        if (!own_cta) segment = (int)quotient(f.inside, in.tiles);
-        in.t = (int)(own_cta ? begin : f.inside - (int64_t)segment * in.tiles);
+        if (apart) f.inside = begin;
+        else segment = (int)quotient(f.inside, in.tiles + kBegin);
+        in.t = (int)(apart ? begin : f.inside - (int64_t)segment * (in.tiles + kBegin)) - kBegin;
+        if (in.t < 0) { in.place = -in.t; in.t = 0; }
         in.head = parts == 1 ? segment : segment / parts;
         in.part = segment - in.head * parts;
         at = in;
@@ -447,6 +476,7 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
             copy_block(ks + h * kBlock * kRow, ks + (kTile + h * kBlock) * kRow, ks + 2 * kTile * kRow + h * 2 * kBlock * 4, in.t * kTile + h * kBlock);
     };
     auto next_tile = [&] {
+        ++in.place;
         if (++in.t < in.tiles) return;
         in.t = 0;
         page_at = page_off = 0;
@@ -730,28 +760,28 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
         }
     };
     float* const early = a.partial + ((int64_t)blockIdx.x * kWarps + warp) * kPiece;
-    bool kept = false;
+    bool kept = false, from_start = at.t == 0;
     if (lane < 2) s_piece[2 * warp + lane].tile0 = -1;
     __syncwarp();
     int to = 0, from = 0;                                                          // stages: of the next copy, of the next tile's work
-    for (int i = 1 - kStages; i < todo; ++i) {
+    for (int i = 1 - kStages; i < 0 || at.place < span; ++i) {
         if (i >= 0) {
             copies_wait<kStages - 2>();
             __syncwarp();
         }
-        if (i < todo - (kStages - 1)) {
+        if (in.place < span) {
             copy_tile(to);
             next_tile();
             to = to + 1 == kStages ? 0 : to + 1;
         }
         copies_end();
         if (i < 0) {
-            if (i == -1 && todo > 0) begin_segment(true);
+            if (i == -1 && at.place < span) begin_segment(true);
             continue;
         }
         work_on(from);
         from = from + 1 == kStages ? 0 : from + 1;
-        const bool ends = at.t + 1 == at.tiles, last = i + 1 == todo;
+        const bool ends = at.t + 1 == at.tiles, last = at.place + 1 + (ends ? kBegin : 0) >= span;
         if (ends || last) {
             const float back = kE4m3 ? __uint_as_float((uint32_t)(value_exp - 6) << 23) : 1.f;
 #pragma unroll
@@ -765,7 +795,7 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
 #pragma unroll
                         for (int c = 0; c < kD / 16; ++c) { o[c][n][j] *= back; o[c][n][2 + j] *= back; }
                 }
-            if (ends && i >= at.t) {                                               // the whole segment was this warp's
+            if (ends && from_start) {                                               // the whole segment was this warp's
 #pragma unroll
                 for (int n = 0; n < kN; ++n) {
                     const float2 inv = at.len > 0 ? float2{reciprocal(l[n][0]), reciprocal(l[n][1])} : float2{0.f, 0.f};
@@ -776,19 +806,21 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
                 }
             } else {
                 if (lane == 0)
-                    s_piece[2 * warp + last] = {begin + i - at.t, at.tiles, at.b, at.head * group + at.part * kHeads, min(kHeads, group - at.part * kHeads)};
+                    s_piece[2 * warp + last] = {begin + at.place - at.t, at.tiles, at.b, at.head * group + at.part * kHeads, min(kHeads, group - at.part * kHeads)};
                 if (last) kept = true;                                             // stays in registers until the rings are done with
                 else keep_piece(false, early);
             }
         }
+        ++at.place;
         if (++at.t == at.tiles) {
             at.t = 0;
-            if (!next_segment(at) && i + 1 < todo) {
+            from_start = true;
+            if (!next_segment(at) && !last) {
                 at.len = within(after_len, most);
                 at.tiles = tiles_of(at.len);
                 if (at.b + 1 < a.batch) after_len = ld_dep(a.lens + at.b + 1);
             }
-            if (i + 1 < todo) begin_segment(false);
+            if (!last) begin_segment(false);
         }
     }
 
@@ -868,7 +900,8 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
         bool last = false;
         if (tid == 0 ? open0 : open1) {
             const Piece p = s_piece[__ffs(tid == 0 ? open0 : open1) - 1];
-            const int c0 = (int)quotient(p.tile0, share), count = (int)quotient(p.tile0 + p.tiles - 1, share) - c0 + 1;
+            const int c0 = apart ? blockIdx.x - own_part : (int)quotient(p.tile0, share);
+            const int count = apart ? own_parts : (int)quotient(p.tile0 + p.tiles - 1, share) - c0 + 1;
             s_cta0[tid] = c0;
             s_ctas[tid] = count;
             last = arrive(a.counters + c0) == count - 1;
@@ -882,43 +915,53 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
         if (!s_last[w]) continue;
         const Piece p = s_piece[__ffs(w == 0 ? open0 : open1) - 1];
         const int c0 = s_cta0[w], count = s_ctas[w];
-        auto piece_of = [&](int i) { return pieces + ((int64_t)(c0 + i) * 2 + (i == 0)) * kOut; };
-        // kSlices threads share a fragment's pieces, kAtOnce of them on their way at a time, the first in front of the weights
+        // the first CTA's piece is its second one, the others' their first
+        const float* const piece0 = pieces + ((int64_t)c0 * 2 + 1) * kOut;
+        const float* const piece1 = pieces + ((int64_t)c0 * 2) * kOut;
+        auto piece_of = [&](int i) { return i == 0 ? piece0 : piece1 + (uint32_t)i * (2 * kOut); };
+        // kSlices threads share a fragment's pieces, kAtOnce of them on their way at a time, the first beside the weights
         constexpr int kSlices = S::kThreads > kUnits ? S::kThreads / kUnits : 1, kPerThread = kUnits > S::kThreads ? kUnits / S::kThreads : 1;
-        constexpr int kAtOnce = S::kThreads > 256 ? 8 : 16;
+        constexpr int kAtOnce = S::kThreads > 256 ? 10 : 20;
         const int slice = tid / kUnits;
-        float4 v[kPerThread];
         uint4 raw[kAtOnce];
         auto ask = [&](int unit, int i0) {
 #pragma unroll
             for (int i = 0; i < kAtOnce; ++i)
                 if (i0 + i * kSlices < count) raw[i] = ld_dep_l2(reinterpret_cast<const uint4*>(piece_of(i0 + i * kSlices)) + unit);
         };
-        ask(tid % kUnits, slice);
+        bool asked = false;
         for (int col = warp; col < kHeads; col += kWarps) {                        // a warp for a query head, a lane for a few CTAs
             float pm[kMaxCtas / 32], pl[kMaxCtas / 32], top = kNone, sum = 0.f;
 #pragma unroll
             for (int i = 0; i < kMaxCtas / 32; ++i) {
                 pm[i] = kNone;
                 pl[i] = 0.f;
-                if (i * 32 + lane < count) {
-                    pm[i] = ld_dep_l2(piece_of(i * 32 + lane) + kPiece + col);
-                    pl[i] = ld_dep_l2(piece_of(i * 32 + lane) + kPiece + kHeads + col);
+                if (i * 32 < count) {
+                    if (i * 32 + lane < count) {
+                        pm[i] = ld_dep_l2(piece_of(i * 32 + lane) + kPiece + col);
+                        pl[i] = ld_dep_l2(piece_of(i * 32 + lane) + kPiece + kHeads + col);
+                    }
                 }
             }
+            if (!asked) ask(tid % kUnits, slice);
+            asked = true;
 #pragma unroll
             for (int i = 0; i < kMaxCtas / 32; ++i) top = fmaxf(top, pm[i]);
             top = warp_max(top);
 #pragma unroll
             for (int i = 0; i < kMaxCtas / 32; ++i) {
-                const float f = exp2_approx(pm[i] - top);
-                sum += f * pl[i];
-                if (i * 32 + lane < count) s_share[i * 32 + lane][col] = f;
+                if (i * 32 < count) {
+                    const float f = exp2_approx(pm[i] - top);
+                    sum += f * pl[i];
+                    if (i * 32 + lane < count) s_share[i * 32 + lane][col] = f;
+                }
             }
             for (int x = 16; x; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
             if (lane == 0) s_inv[col] = reciprocal(sum);
         }
+        if (!asked) ask(tid % kUnits, slice);
         __syncthreads();
+        float4 v[kPerThread];
 #pragma unroll
         for (int k = 0; k < kPerThread; ++k) {
             const int unit = (tid + k * S::kThreads) % kUnits, col = (unit >> 5) % kN * 8 + 2 * t4;
