@@ -314,15 +314,17 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
             cta0 = blockIdx.x * share;
             cta1 = cta0 + share < total ? cta0 + share : total;
             if (cta0 >= total) return;
-            if (longest <= 2 * kWarps) {
-                auto rounded = [&](int64_t place) {                               // to the nearer end of its segment
-                    if (place >= total) return total;
+            if (longest <= 2 * kWarps) {                                          // ... to the nearer end of a segment
+#pragma unroll 1
+                for (int side = 0; side < 2; ++side) {
+                    const int64_t place = side == 0 ? cta0 : cta1;
+                    if (place >= total) break;
                     const Found f = find(places_of, before, mine, place);
                     const int places = tiles_of(f.len) + kBegin, in_segment = (int)(f.inside - quotient(f.inside, places) * places);
-                    return place + (2 * in_segment < places ? -in_segment : places - in_segment);
-                };
-                cta0 = rounded(cta0);
-                cta1 = rounded(cta1);
+                    const int64_t moved = place + (2 * in_segment < places ? -in_segment : places - in_segment);
+                    if (side == 0) cta0 = moved;
+                    else cta1 = moved;
+                }
                 if (cta0 >= cta1) return;
             }
         }
