@@ -8,40 +8,90 @@
 // A NaN or an infinity in a row makes its scale one, and with it everything that is read back of the row.
 // Both are bound by memory: 2 D bytes in and D + 4 (or 2 D) bytes out per row, and the other way round.
 //
-// A lane holds 16 channels of a row (32 bytes of bf16, 16 of codes), the lanes of a row lie side by side (2 .. 16 of them, a
-// power of two, so that a row's maximum is a few shuffles), and a thread has kDeep rows in flight.  A block takes a few tokens
-// with all their heads, keys and values: what a token needs (its slot; its sequence, page and offset) is looked up once per block.
+// The lanes of a row lie side by side (2 .. 16 of them, a power of two, so that a row's maximum is a few shuffles).  Of bf16 a lane holds two
+// words of eight channels, one in either half of the row, so that every load and store of a row's lanes is one stretch; of codes it
+// holds 16, even lanes in the row's first half and odd ones in its second, and neighbours exchange half of theirs on the way.
+// (Reading 206 MB back took 46 us with a lane's 16 channels side by side on both sides, which writes half sectors, and 50 with two
+// times eight codes a lane.)
+// A thread has kDeep rows in flight: four, or one where the call has no more for it (2.3 instead of 3.4 us for 64 tokens of 4 heads).  A block takes a few tokens at a time with all their heads, keys and values; what a token needs (its slot; its
+// sequence, page and offset) is looked up once, a turn early: looked up when it was needed, it took longer than the rows.
 #include "common.cuh"
 #include "kernels.h"
 
 namespace fp8lin {
 
 constexpr int kCacheThreads = 256;
-constexpr int kDeep = 4;              // rows that a thread has in flight
-constexpr int kMaxTokens = 64;        // tokens of a block
+constexpr int kMaxTokens = 64;        // tokens of a block's turn
+constexpr int kCacheBlocks = 8;       // blocks of a launch per SM, twice what it holds at a time
+constexpr int kMaxEnds = 1024;        // sequences whose ends fit a block's shared memory
 
 struct CacheGrid {
     int lanes_log2;                   // lanes of a row
-    int tokens;                       // tokens of a block
+    int tokens;                       // tokens of a block's turn
+    int64_t turns;                    // of all blocks
+    int blocks;
 };
 
-// Rows of a block, one behind the other: token, keys then values, head.
+// Rows of a block, one behind the other: token, keys then values, head.  A thread goes through them in steps of as many as the block takes at a time.
 struct RowAt {
-    int token, head;
-    bool values;
+    int token, rest;
+    __device__ __forceinline__ RowAt(int row, int rows_of_token) : token(row / rows_of_token), rest(row - token * rows_of_token) {}
+    __device__ __forceinline__ void step(int tokens, int more, int rows_of_token) {
+        token += tokens;
+        rest += more;
+        if (rest >= rows_of_token) { rest -= rows_of_token; ++token; }
+    }
 };
-__device__ __forceinline__ RowAt row_at(int row, int heads) {
-    const int token = row / (2 * heads), rest = row - token * 2 * heads;
-    const bool values = rest >= heads;
-    return {token, values ? rest - heads : rest, values};
-}
+// ... and what it reads and writes there: the head's place in the cache and the row outside it, which only moves from token to
+// token where a step is one of whole tokens.
+struct CacheLane {
+    int tid, sub, step, heads, chunks, lanes;
+    RowAt at, steps;
+    unsigned char* cache;             // of the head, in token 0's place
+    float* scales;
+    __nv_bfloat16* row;               // outside the cache
+    int64_t row_step;                 // a step of `steps.token` tokens, where heads stay
+    __device__ __forceinline__ CacheLane(const CacheView& c, const CacheRows& x, const CacheGrid& grid)
+        : tid(threadIdx.x), sub(tid & ((1 << grid.lanes_log2) - 1)), step(kCacheThreads >> grid.lanes_log2), heads(c.kv_heads), chunks(c.dim >> 3),
+          lanes(1 << grid.lanes_log2), at(tid >> grid.lanes_log2, 2 * c.kv_heads), steps(step, 2 * c.kv_heads) {}
+    __device__ __forceinline__ void place(const CacheView& c, const CacheRows& x, int64_t token0) {
+        const bool values = at.rest >= heads;
+        const int head = values ? at.rest - heads : at.rest;
+        cache = (values ? c.v : c.k) + head * c.sh;
+        scales = (values ? c.v_scale : c.k_scale) + head * c.ssh;
+        row = (values ? x.v : x.k) + (token0 + at.token) * (values ? x.vt : x.kt) + head * (values ? x.vh : x.kh);
+        row_step = steps.token * (values ? x.vt : x.kt);
+    }
+    __device__ __forceinline__ void next(const CacheView& c, const CacheRows& x, int64_t token0) {
+        at.step(steps.token, steps.rest, 2 * heads);
+        if (steps.rest == 0) row += row_step;
+        else place(c, x, token0);
+    }
+};
 
-__device__ __forceinline__ uint32_t max_bits(uint4 w) {
-    const uint32_t m = __vmaxu2(__vmaxu2(w.x & 0x7fff7fffu, w.y & 0x7fff7fffu), __vmaxu2(w.z & 0x7fff7fffu, w.w & 0x7fff7fffu));
-    return max(m & 0xffffu, m >> 16);
+__device__ __forceinline__ uint2 neighbours(uint2 x) { return {__shfl_xor_sync(0xffffffffu, x.x, 1), __shfl_xor_sync(0xffffffffu, x.y, 1)}; }
+
+// The larger magnitudes of two pairs of bf16 numbers (a NaN is the largest); the signs are of no use.
+__device__ __forceinline__ uint32_t max_abs2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.NaN.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
 }
-// x / s where s is an infinity or a NaN: a zero of x's sign, or a NaN
-__device__ __forceinline__ uint2 quant8_not_finite(uint4 w, float s) {
+// x / s for eight values where neither quotients nor what leads to them can overflow: a quotient refined as in ExactDiv, but of -x, whose
+// codes are then negated; computed that way zeros keep their signs.  (nr, s: -1 / s and s, twice)
+__device__ __forceinline__ uint2 quant8_finite(uint4 v, uint64_t nr, uint64_t s) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    uint32_t c[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint64_t x = pack_f32x2(bf16_lo(w[i]), bf16_hi(w[i]));
+        const uint64_t q0 = mul_f32x2(x, nr);
+        c[i] = cvt_e4m3x2(fma_f32x2(fma_f32x2(q0, s, x), nr, q0));
+    }
+    return {(c[0] | (c[1] << 16)) ^ 0x80808080u, (c[2] | (c[3] << 16)) ^ 0x80808080u};
+}
+// ... and in general; where s is an infinity or a NaN: a zero of x's sign, or a NaN
+__device__ __forceinline__ uint2 quant8_any(uint4 w, float s) {
     const uint32_t v[4] = {w.x, w.y, w.z, w.w};
     uint32_t q[4];
 #pragma unroll
@@ -49,194 +99,257 @@ __device__ __forceinline__ uint2 quant8_not_finite(uint4 w, float s) {
     return {q[0] | (q[1] << 16), q[2] | (q[3] << 16)};
 }
 
-template <bool kE4m3>
-__global__ void __launch_bounds__(kCacheThreads)
-kv_cache_write_kernel(CacheView c, CacheRows x, const int* slots, CacheGrid grid, int* status) {
-    __shared__ int64_t s_at[kMaxTokens], s_scale_at[kMaxTokens];        // where a token lies in the cache, -1: nowhere
-    pdl_launch_dependents();
-    pdl_wait();
-    const int tid = threadIdx.x, sub = tid & ((1 << grid.lanes_log2) - 1), lanes_log2 = grid.lanes_log2;
-    const int64_t token0 = (int64_t)blockIdx.x * grid.tokens;
-    const int tokens = x.rows - token0 < grid.tokens ? (int)(x.rows - token0) : grid.tokens;
-    const int rows = tokens * 2 * c.kv_heads, step = kCacheThreads >> lanes_log2;
-    const bool mine = sub * 16 < c.dim;
-    if (tid < tokens) {
-        const int slot = ld_dep(slots + token0 + tid);
-        const int64_t page = slot / c.block_size, off = slot - page * c.block_size;
-        const bool there = slot >= 0 && page < c.num_blocks;
-        if (slot >= 0 && !there) report_status(status, kDevBadPage);
-        s_at[tid] = there ? page * c.sb + off * c.st : -1;
-        s_scale_at[tid] = page * c.ssb + off * c.sst;
+// Where a token lies in the cache: byte offset of its rows, element offset of its scales; -1: nowhere.
+struct TokenAt {
+    int64_t row, scale;
+};
+__device__ __forceinline__ TokenAt token_at(const CacheView& c, int64_t page, int64_t off, int* status) {
+    if (page < 0 || page >= c.num_blocks) {
+        report_status(status, kDevBadPage);
+        return {-1, -1};
     }
-    for (int turn = 0; turn < rows; turn += step * kDeep) {             // (as many for every thread: a row's lanes meet below)
-        uint4 w[kDeep][2];
-        RowAt at[kDeep];
+    return {page * c.sb + off * c.st, page * c.ssb + off * c.sst};
+}
+
+template <bool kE4m3, int kDeep>
+__global__ void __launch_bounds__(kCacheThreads, kDeep == 1 ? 6 : 4)
+kv_cache_write_kernel(CacheView c, CacheRows x, const int* slots, CacheGrid grid, int* status) {
+    __shared__ TokenAt s_at[2][kMaxTokens];
+    pdl_launch_dependents();
+    const CacheLane origin(c, x, grid);
+    const int word0 = origin.sub, word1 = origin.sub + origin.lanes;     // of eight bf16 channels
+    const bool low = word0 < origin.chunks, high = word1 < origin.chunks, odd = origin.sub & 1;
+    const int code = (origin.sub >> 1) + (odd ? origin.lanes >> 1 : 0);  // of 16 codes
+    pdl_wait();
+    auto tokens_of = [&](int64_t turn) {
+        const int64_t left = x.rows - turn * grid.tokens;
+        return left < grid.tokens ? (int)left : grid.tokens;
+    };
+    auto slot_of = [&](int64_t turn) { return turn < grid.turns && origin.tid < tokens_of(turn) ? ld_dep(slots + turn * grid.tokens + origin.tid) : -1; };
+    auto put = [&](int slot, int side) {
+        if (origin.tid >= kMaxTokens) return;
+        const int64_t page = slot / c.block_size;
+        s_at[side][origin.tid] = slot < 0 ? TokenAt{-1, -1} : token_at(c, page, slot - page * c.block_size, status);
+    };
+    int slot = slot_of(blockIdx.x), side = 0;
+    bool placed = false;
+    for (int64_t turn = blockIdx.x; turn < grid.turns; turn += gridDim.x, side ^= 1) {
+        const int64_t token0 = turn * grid.tokens;
+        const int tokens = tokens_of(turn), rows = tokens * 2 * c.kv_heads;
+        CacheLane me = origin;
+        me.place(c, x, token0);
+        for (int row0 = 0; row0 < rows; row0 += me.step * kDeep) {       // (as often for every thread: a row's lanes meet below)
+            uint4 w[kDeep][2];
+            CacheLane it = me;
 #pragma unroll
-        for (int i = 0; i < kDeep; ++i) {
-            const int row = turn + (tid >> lanes_log2) + i * step;
-            at[i] = row_at(row, c.kv_heads);
-            w[i][0] = w[i][1] = {0, 0, 0, 0};
-            if (row < rows && mine) {
-                const int64_t t = token0 + at[i].token;
-                const uint4* src = reinterpret_cast<const uint4*>(at[i].values ? x.v + t * x.vt + at[i].head * x.vh : x.k + t * x.kt + at[i].head * x.kh) + 2 * sub;
-                w[i][0] = ld_dep(src);
-                w[i][1] = ld_dep(src + 1);
-            }
-        }
-        if (turn == 0) __syncthreads();               // the slots, asked for before the rows
-#pragma unroll
-        for (int i = 0; i < kDeep; ++i) {
-            const int row = turn + (tid >> lanes_log2) + i * step;
-            const int64_t to = row < rows ? s_at[at[i].token] : -1;
-            unsigned char* dst = (at[i].values ? c.v : c.k) + to + at[i].head * c.sh;
-            if (!kE4m3) {
-                if (to >= 0 && mine) {
-                    reinterpret_cast<uint4*>(dst)[2 * sub] = w[i][0];
-                    reinterpret_cast<uint4*>(dst)[2 * sub + 1] = w[i][1];
+            for (int i = 0; i < kDeep; ++i, it.next(c, x, token0)) {
+                w[i][0] = w[i][1] = {0, 0, 0, 0};
+                if (it.at.token < tokens) {
+                    const uint4* src = reinterpret_cast<const uint4*>(it.row);
+                    if (low) w[i][0] = ld_dep(src + word0);
+                    if (high) w[i][1] = ld_dep(src + word1);
                 }
-                continue;
             }
-            // |x| as its bits: ordered as the values are, a NaN above the infinity
-            uint32_t m = max(max_bits(w[i][0]), max_bits(w[i][1]));
-            for (int o = 1; o < 1 << lanes_log2; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-            if (to < 0) continue;
-            const float top = __uint_as_float(m << 16), s = __fdiv_rn(m > 0x7f80u ? top : fmaxf(top, 1e-8f), 448.f);
-            if (mine) {
-                uint2 lo, hi;
-                if (m < 0x7f80u) {
-                    const ExactDiv div(s);
-                    lo = quant8_e4m3(w[i][0], div);
-                    hi = quant8_e4m3(w[i][1], div);
+            if (!placed) {                                               // the first slots, asked for in front of the rows
+                put(slot, side);
+                placed = true;
+                __syncthreads();
+            }
+            if (row0 == 0) slot = slot_of(turn + gridDim.x);
+#pragma unroll
+            for (int i = 0; i < kDeep; ++i, me.next(c, x, token0)) {
+                const TokenAt to = me.at.token < tokens ? s_at[side][me.at.token] : TokenAt{-1, -1};
+                unsigned char* dst = me.cache + to.row;
+                if (!kE4m3) {
+                    if (to.row >= 0 && low) reinterpret_cast<uint4*>(dst)[word0] = w[i][0];
+                    if (to.row >= 0 && high) reinterpret_cast<uint4*>(dst)[word1] = w[i][1];
+                    continue;
+                }
+                // |x| as its bits: ordered as the values are, a NaN above the infinity
+                const uint4 &a = w[i][0], &b = w[i][1];
+                const uint32_t m2 = max_abs2(max_abs2(max_abs2(a.x, a.y), max_abs2(a.z, a.w)), max_abs2(max_abs2(b.x, b.y), max_abs2(b.z, b.w)));
+                uint32_t m = max(m2 & 0x7fffu, (m2 >> 16) & 0x7fffu);
+                for (int o = 1; o < me.lanes; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+                // top / 448, correctly rounded as in ExactDiv (where top is not finite, the first product is the answer)
+                const float top = m > 0x7f80u ? __uint_as_float(m << 16) : fmaxf(__uint_as_float(m << 16), 1e-8f), r448 = 1.f / 448.f, q0 = top * r448;
+                const float s = m < 0x7f80u ? fmaf(fmaf(-q0, 448.f, top), r448, q0) : q0;
+                uint2 c0, c1;
+                if (top < 1e38f) {                                      // quotients are 448 at most, and what leads to them is no larger than top
+                    const float r = __frcp_rn(s);
+                    const uint64_t nr = pack_f32x2(-r, -r), ss = pack_f32x2(s, s);
+                    c0 = quant8_finite(a, nr, ss);
+                    c1 = quant8_finite(b, nr, ss);
                 } else {
-                    lo = quant8_not_finite(w[i][0], s);
-                    hi = quant8_not_finite(w[i][1], s);
+                    c0 = quant8_any(a, s);
+                    c1 = quant8_any(b, s);
                 }
-                reinterpret_cast<uint4*>(dst)[sub] = {lo.x, lo.y, hi.x, hi.y};
+                const uint2 got = neighbours(odd ? c0 : c1);
+                if (to.row >= 0) {
+                    if (code * 2 < me.chunks) reinterpret_cast<uint4*>(dst)[code] = odd ? uint4{got.x, got.y, c1.x, c1.y} : uint4{c0.x, c0.y, got.x, got.y};
+                    if (me.sub == 0) me.scales[to.scale] = s;
+                }
             }
-            if (sub == 0) (at[i].values ? c.v_scale : c.k_scale)[s_scale_at[at[i].token] + at[i].head * c.ssh] = s;
         }
+        put(slot, side ^ 1);
+        __syncthreads();
     }
 }
 
 // The sequence b with cu[b] <= row < cu[b + 1], or -1.
-__device__ __forceinline__ int sequence_of(const int* cu, int batch, int64_t row) {
+template <class Ends>
+__device__ __forceinline__ int sequence_of(Ends cu, int batch, int64_t row) {
     int lo = 0, hi = batch;                        // cu[lo] <= row < cu[hi], if there is one
-    if (row < ld_dep(cu) || row >= ld_dep(cu + batch)) return -1;
+    if (row < cu(0) || row >= cu(batch)) return -1;
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
-        if (ld_dep(cu + mid) <= row) lo = mid;
+        if (cu(mid) <= row) lo = mid;
         else hi = mid;
     }
     return lo;
 }
 
-template <bool kE4m3>
-__global__ void __launch_bounds__(kCacheThreads)
+template <bool kE4m3, int kDeep>
+__global__ void __launch_bounds__(kCacheThreads, kDeep == 1 ? 6 : 4)
 kv_cache_read_kernel(CacheView c, CacheRows y, const int* tables, int64_t ld_tables, int64_t max_pages, const int* cu, int batch, CacheGrid grid, int* status) {
-    __shared__ int64_t s_at[kMaxTokens], s_scale_at[kMaxTokens];
+    __shared__ TokenAt s_at[2][kMaxTokens];
+    __shared__ int s_ends[kMaxEnds + 1];
     pdl_launch_dependents();
+    const CacheLane origin(c, y, grid);
+    const int tid = origin.tid;
+    const int word0 = origin.sub, word1 = origin.sub + origin.lanes;     // of eight bf16 channels
+    const bool low = word0 < origin.chunks, high = word1 < origin.chunks, odd = origin.sub & 1;
+    const int code = (origin.sub >> 1) + (odd ? origin.lanes >> 1 : 0);  // of 16 codes
     pdl_wait();
-    const int tid = threadIdx.x, sub = tid & ((1 << grid.lanes_log2) - 1), lanes_log2 = grid.lanes_log2;
-    const int64_t token0 = (int64_t)blockIdx.x * grid.tokens;
-    const int tokens = y.rows - token0 < grid.tokens ? (int)(y.rows - token0) : grid.tokens;
-    const int rows = tokens * 2 * c.kv_heads, step = kCacheThreads >> lanes_log2;
-    if (tid < tokens) {
-        const int64_t row = token0 + tid;
-        const int b = sequence_of(cu, batch, row);
-        int64_t page = -1, off = 0;
-        if (b >= 0) {
-            const int64_t at = row - ld_dep(cu + b), i = at / c.block_size;
-            off = at - i * c.block_size;
-            if (i < max_pages) page = ld_dep(tables + b * ld_tables + i);
-            if (page < 0 || page >= c.num_blocks) {
-                page = -1;
-                report_status(status, kDevBadPage);
-            }
-        }
-        s_at[tid] = page < 0 ? -1 : page * c.sb + off * c.st;
-        s_scale_at[tid] = page * c.ssb + off * c.sst;
-    }
+    if (batch <= kMaxEnds)
+        for (int i = tid; i <= batch; i += kCacheThreads) s_ends[i] = ld_dep(cu + i);
     __syncthreads();
-    if (sub * 16 >= c.dim) return;
-    for (int row0 = tid >> lanes_log2; row0 < rows; row0 += step * kDeep) {
-        uint4 w[kDeep][2];
-        float s[kDeep];
-        RowAt at[kDeep];
-        bool there[kDeep];
+    // A token's page and offset; the page on its way.
+    struct Looked { int64_t off; int page; bool there; };
+    auto look = [&](int64_t turn) {
+        Looked l = {0, -1, false};
+        const int64_t row = turn * grid.tokens + tid;
+        if (turn >= grid.turns || tid >= grid.tokens || row >= y.rows) return l;
+        int b;
+        int64_t at;
+        if (batch <= kMaxEnds) {
+            b = sequence_of([&](int i) { return s_ends[i]; }, batch, row);
+            at = b < 0 ? 0 : row - s_ends[b];
+        } else {
+            b = sequence_of([&](int i) { return ld_dep(cu + i); }, batch, row);
+            at = b < 0 ? 0 : row - ld_dep(cu + b);
+        }
+        if (b < 0) return l;
+        const int64_t i = at / c.block_size;
+        l.off = at - i * c.block_size;
+        l.there = true;
+        if (i < max_pages) l.page = ld_dep(tables + b * ld_tables + i);
+        return l;
+    };
+    auto put = [&](const Looked& l, int side) {
+        if (tid < kMaxTokens) s_at[side][tid] = l.there ? token_at(c, l.page, l.off, status) : TokenAt{-1, -1};
+    };
+    int side = 0;
+    put(look(blockIdx.x), side);
+    __syncthreads();
+    for (int64_t turn = blockIdx.x; turn < grid.turns; turn += gridDim.x, side ^= 1) {
+        const int64_t token0 = turn * grid.tokens;
+        const int tokens = y.rows - token0 < grid.tokens ? (int)(y.rows - token0) : grid.tokens;
+        const Looked next = look(turn + gridDim.x);
+        CacheLane me = origin;
+        me.place(c, y, token0);
+        for (int row0 = 0; row0 < tokens * 2 * c.kv_heads; row0 += me.step * kDeep) {      // (as often for every thread: neighbours meet below)
+            uint4 w[kDeep][2] = {};
+            float s[kDeep] = {};
+            CacheLane it = me;
+            bool there[kDeep];
 #pragma unroll
-        for (int i = 0; i < kDeep; ++i) {
-            const int row = row0 + i * step;
-            at[i] = row_at(row, c.kv_heads);
-            const int64_t from = row < rows ? s_at[at[i].token] : -1;
-            there[i] = from >= 0;
-            if (there[i]) {
-                const uint4* src = reinterpret_cast<const uint4*>((at[i].values ? c.v : c.k) + from + at[i].head * c.sh);
+            for (int i = 0; i < kDeep; ++i, it.next(c, y, token0)) {
+                const TokenAt from = it.at.token < tokens ? s_at[side][it.at.token] : TokenAt{-1, -1};
+                there[i] = from.row >= 0;
+                if (there[i]) {
+                    const unsigned char* src = it.cache + from.row;
+                    if (kE4m3) {
+                        if (code * 2 < it.chunks) w[i][0] = ld_dep(reinterpret_cast<const uint4*>(src) + code);
+                        s[i] = ld_dep(it.scales + from.scale);
+                    } else {
+                        if (low) w[i][0] = ld_dep(reinterpret_cast<const uint4*>(src) + word0);
+                        if (high) w[i][1] = ld_dep(reinterpret_cast<const uint4*>(src) + word1);
+                    }
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < kDeep; ++i, me.next(c, y, token0)) {
+                uint4* dst = reinterpret_cast<uint4*>(me.row);
                 if (kE4m3) {
-                    w[i][0] = ld_dep(src + sub);
-                    s[i] = ld_dep((at[i].values ? c.v_scale : c.k_scale) + s_scale_at[at[i].token] + at[i].head * c.ssh);
-                } else {
-                    w[i][0] = ld_dep(src + 2 * sub);
-                    w[i][1] = ld_dep(src + 2 * sub + 1);
+                    const uint64_t ss = pack_f32x2(s[i], s[i]);
+                    auto widened = [&](uint32_t x, uint32_t z) {         // eight codes
+                        uint32_t o[4];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const uint32_t h = cvt_e4m3x2_to_f16x2((uint16_t)((j < 2 ? x : z) >> (16 * (j & 1))));
+                            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+                            float lo, hi;
+                            unpack_f32x2(mul_f32x2(pack_f32x2(f.x, f.y), ss), lo, hi);
+                            o[j] = pack_bf16x2(lo, hi);
+                        }
+                        return uint4{o[0], o[1], o[2], o[3]};
+                    };
+                    const uint2 c0 = {w[i][0].x, w[i][0].y}, c1 = {w[i][0].z, w[i][0].w}, got = neighbours(odd ? c0 : c1);
+                    if (there[i] && low) dst[word0] = odd ? widened(got.x, got.y) : widened(c0.x, c0.y);
+                    if (there[i] && high) dst[word1] = odd ? widened(c1.x, c1.y) : widened(got.x, got.y);
+                } else if (there[i]) {
+                    if (low) dst[word0] = w[i][0];
+                    if (high) dst[word1] = w[i][1];
                 }
             }
         }
-#pragma unroll
-        for (int i = 0; i < kDeep; ++i) {
-            if (!there[i]) continue;
-            const int64_t t = token0 + at[i].token;
-            uint4* dst = reinterpret_cast<uint4*>(at[i].values ? y.v + t * y.vt + at[i].head * y.vh : y.k + t * y.kt + at[i].head * y.kh) + 2 * sub;
-            if (kE4m3) {
-                const uint32_t v[4] = {w[i][0].x, w[i][0].y, w[i][0].z, w[i][0].w};
-                uint32_t o[8];
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const uint32_t h = cvt_e4m3x2_to_f16x2((uint16_t)(v[j >> 1] >> (16 * (j & 1))));
-                    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
-                    o[j] = pack_bf16x2(f.x * s[i], f.y * s[i]);
-                }
-                dst[0] = {o[0], o[1], o[2], o[3]};
-                dst[1] = {o[4], o[5], o[6], o[7]};
-            } else {
-                dst[0] = w[i][0];
-                dst[1] = w[i][1];
-            }
-        }
+        put(next, side ^ 1);
+        __syncthreads();
     }
 }
 
-// Tokens of a block: as many as its threads take in one turn of kDeep rows; fewer where that would leave SMs without a block.
-static CacheGrid cache_grid(const CacheView& c, int64_t rows) {
-    CacheGrid g = {0, 1};
+// Tokens of a block's turn: as many as its threads take at once, `deep` rows each; fewer where that would leave SMs without a block.
+static CacheGrid cache_grid(const CacheView& c, int64_t rows, int deep) {
+    CacheGrid g = {1, 1, 0, 0};
     while ((16 << g.lanes_log2) < c.dim) ++g.lanes_log2;
-    const int at_once = (kCacheThreads >> g.lanes_log2) * kDeep / (2 * c.kv_heads);
+    const int at_once = (kCacheThreads >> g.lanes_log2) * deep / (2 * c.kv_heads);
     while (g.tokens < kMaxTokens && 2 * g.tokens <= at_once && rows > (int64_t)g.tokens * sm_count()) g.tokens *= 2;
+    g.turns = (rows + g.tokens - 1) / g.tokens;
+    const int64_t most = (int64_t)kCacheBlocks * sm_count();
+    g.blocks = (int)(g.turns < most ? g.turns : most);
     return g;
 }
 
-cudaError_t launch_kv_cache_write(const CacheView& c, const CacheRows& x, const int* slots, int* status, cudaStream_t stream) {
-    const CacheGrid g = cache_grid(c, x.rows);
+// Whether four rows a thread would leave some without any: the chip's threads hold the call's rows once.
+static bool few_rows(const CacheView& c, int64_t rows) {
+    return rows * 2 * c.kv_heads <= (int64_t)sm_count() * 4 * (kCacheThreads >> cache_grid(c, rows, 1).lanes_log2);
+}
+
+template <class Kernel, class... Args>
+static cudaError_t launch_cache(Kernel kernel, int blocks, cudaStream_t stream, Args... args) {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)((x.rows + g.tokens - 1) / g.tokens));
+    cfg.gridDim = dim3((unsigned)blocks);
     cfg.blockDim = dim3(kCacheThreads);
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     cfg.numAttrs = pdl_attribute(attr);
     cfg.attrs = attr;
-    return counted(cudaLaunchKernelEx(&cfg, c.e4m3 ? kv_cache_write_kernel<true> : kv_cache_write_kernel<false>, c, x, slots, g, status));
+    return counted(cudaLaunchKernelEx(&cfg, kernel, args...));
+}
+
+cudaError_t launch_kv_cache_write(const CacheView& c, const CacheRows& x, const int* slots, int* status, cudaStream_t stream) {
+    const bool few = few_rows(c, x.rows);
+    const CacheGrid g = cache_grid(c, x.rows, few ? 1 : 4);
+    auto kernel = c.e4m3 ? (few ? kv_cache_write_kernel<true, 1> : kv_cache_write_kernel<true, 4>) : (few ? kv_cache_write_kernel<false, 1> : kv_cache_write_kernel<false, 4>);
+    return launch_cache(kernel, g.blocks, stream, c, x, slots, g, status);
 }
 
 cudaError_t launch_kv_cache_read(const CacheView& c, const CacheRows& y, const int* tables, int64_t ld_tables, int64_t max_pages, const int* cu_seqlens,
                                  int64_t batch, int* status, cudaStream_t stream) {
-    const CacheGrid g = cache_grid(c, y.rows);
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)((y.rows + g.tokens - 1) / g.tokens));
-    cfg.blockDim = dim3(kCacheThreads);
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    cfg.numAttrs = pdl_attribute(attr);
-    cfg.attrs = attr;
-    return counted(cudaLaunchKernelEx(&cfg, c.e4m3 ? kv_cache_read_kernel<true> : kv_cache_read_kernel<false>, c, y, tables, ld_tables, max_pages, cu_seqlens,
-                                      (int)batch, g, status));
+    const bool few = few_rows(c, y.rows);
+    const CacheGrid g = cache_grid(c, y.rows, few ? 1 : 4);
+    auto kernel = c.e4m3 ? (few ? kv_cache_read_kernel<true, 1> : kv_cache_read_kernel<true, 4>) : (few ? kv_cache_read_kernel<false, 1> : kv_cache_read_kernel<false, 4>);
+    return launch_cache(kernel, g.blocks, stream, c, y, tables, ld_tables, max_pages, cu_seqlens, (int)batch, g, status);
 }
 
 }  // namespace fp8lin
