@@ -108,6 +108,7 @@ int fp8lin_paged_attention(const fp8lin_kv_cache* cache, const void* q, int64_t 
     if (int rc = check_tables(block_tables, ld_tables, max_pages, batch)) return rc;
     if (num_heads <= 0 || num_heads % a.c.kv_heads != 0 || num_heads > 65535)
         return set_error(FP8LIN_ERR_SHAPE, "num_heads=%lld must be a multiple of num_kv_heads=%d", (long long)num_heads, a.c.kv_heads);
+    if (batch * num_heads > 0x7fffffff) return set_error(FP8LIN_ERR_SHAPE, "batch=%lld times num_heads=%lld is too large", (long long)batch, (long long)num_heads);
     if (batch == 0) return FP8LIN_OK;
     if (!q || !context_lens || !out) return set_error(FP8LIN_ERR_NULL, "q, context_lens and out must not be NULL");
     if (!aligned16(q) || bad_stride(q_stride_row, batch, 8) || bad_stride(q_stride_head, num_heads, 8))

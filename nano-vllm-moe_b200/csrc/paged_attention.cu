@@ -33,6 +33,8 @@ namespace {
 
 constexpr int kBlock = 16;                      // tokens of a matrix instruction
 constexpr int kMaxCtas = 192;                   // of a launch: one per SM
+constexpr int kJoin = 16;                       // pieces that a CTA joins at a time
+static_assert(3 * kMaxCtas <= kWsMaxCounters, "counters: two per CTA for its pieces, one for a segment's second step");
 constexpr float kLog2e = 1.4426950408889634f;
 
 template <bool kE4m3_, int kD_, int kN_, int kM_, int kWarps_, int kStages_>
@@ -205,9 +207,9 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
     extern __shared__ __align__(1024) unsigned char ring[];
     __shared__ Piece s_piece[2 * kWarps];
     // (read two heads at a time)
-    __shared__ __align__(16) float s_m[2 * kWarps][kHeads], s_l[2 * kWarps][kHeads], s_f[2 * kWarps][kHeads], s_inv[kHeads], s_share[kMaxCtas][kHeads];
+    __shared__ __align__(16) float s_m[2 * kWarps][kHeads], s_l[2 * kWarps][kHeads], s_f[2 * kWarps][kHeads], s_top[kHeads], s_sum[kHeads], s_share[kJoin][kHeads];
     __shared__ int s_entry[2 * kWarps];                                          // the pieces that there are, in the order of the list
-    __shared__ int s_last[2], s_cta0[2], s_ctas[2];                              // segments that other CTAs have pieces of; which CTAs
+    __shared__ int s_last[2], s_cta0[2], s_ctas[2], s_again;                     // segments that other CTAs have pieces of; which CTAs
 
     auto tiles_of = [](int len) { return tiles_in<kTile>(len); };
     pdl_launch_dependents();
@@ -337,7 +339,8 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
     unsigned char* const my_ring = ring + warp * (kStages * S::kStageBytes);
     const uint32_t my_ring_at = smem_addr(my_ring);
     const int row_bytes = a.c.dim * (kE4m3 ? 1 : 2);
-    const bool paged16 = a.c.block_size % kBlock == 0;
+    const int page_size = a.c.block_size, page_magic = page_size <= kBlock ? 65536 / page_size + 1 : 0;
+    auto pages_in = [&](int tokens) { return page_size > kBlock ? (tokens >= page_size ? 1 : 0) : tokens * page_magic >> 16; };      // up to 30 tokens, or less than two pages
     const int g = lane >> 2, t4 = lane & 3;
     if (row_bytes < kRow) {                                         // channels behind head_dim: zeros once, they are never copied to
         for (int i = lane * 16; i < kStages * S::kStageBytes; i += 512) *reinterpret_cast<uint4*>(my_ring + i) = {0, 0, 0, 0};
@@ -346,7 +349,7 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
 
     struct Place {
         int b, head, part, t, len, tiles, place;                    // sequence, key head, part of its query heads, tile; its place from `begin` on
-    } in, at;                                                       // of the next tile to copy, and to work on
+    } in = {}, at = {};                                             // of the next tile to copy, and to work on
     auto next_segment = [&](Place& x) {                             // whether it is one of the same sequence
         x.place += kBegin;
         if (++x.part < parts) return true;
@@ -357,18 +360,17 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
         return false;
     };
     // Nothing that the loop needs is waited for in it: a load queues behind all the copies that the SM's warps have asked for, some 2.5 us.  So lengths and
-    // queries are asked for a segment early, and pages (where they hold whole blocks) come 32 table entries at a time, a lane each, also early: those from
-    // page_base on, the 32 behind them, a sequence's first for its next head, and the next sequence's.
+    // queries are asked for a segment early, and pages come 32 table entries at a time, a lane each, also early: those from page_base on, the 32 behind
+    // them, a sequence's first for its next head, and the next sequence's.
     int pages = 0, pages_behind = 0, pages_first = 0, page_base = 0, page_at = 0, page_off = 0;
     int next_len = 0, next_pages = 0, after_len = 0;                // of the sequences behind in.b, behind at.b
-    auto entry = [&](int b, int64_t i) { return paged16 && i < a.max_pages ? ld_dep(a.tables + (int64_t)b * a.ld_tables + i) : -1; };
+    auto entry = [&](int b, int64_t i) { return i < a.max_pages ? ld_dep(a.tables + (int64_t)b * a.ld_tables + i) : -1; };
     auto look_at = [&](int b) {
         if (b < a.batch) {
             next_len = ld_dep(a.lens + b);
             next_pages = entry(b, lane);
         }
     };
-    in.place = at.place = 0;
     if (span > 0) {
         Found f = own;
         int segment = own_segment;
@@ -383,13 +385,11 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
         in.head = parts == 1 ? segment : segment / parts;
         in.part = segment - in.head * parts;
         at = in;
-        if (paged16) {
-            page_base = page_at = in.t * kTile / a.c.block_size;
-            page_off = in.t * kTile - page_at * a.c.block_size;
-            pages = entry(in.b, page_base + lane);
-            pages_behind = entry(in.b, page_base + 32 + lane);
-            pages_first = entry(in.b, lane);
-        }
+        page_base = page_at = in.t * kTile / page_size;
+        page_off = in.t * kTile - page_at * page_size;
+        pages = entry(in.b, page_base + lane);
+        pages_behind = entry(in.b, page_base + 32 + lane);
+        pages_first = entry(in.b, lane);
         look_at(in.b + 1);
         if (at.b + 1 < a.batch) after_len = ld_dep(a.lens + at.b + 1);
     }
@@ -404,18 +404,17 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
     auto copy_block = [&](uint32_t ks, uint32_t vs, uint32_t scales, int token0) {
         const int rows = in.len - token0;                                         // that exist: at least 16, but at a sequence's end
         auto dst_of = [&](int j) { return j * S::kRowsPerCopy * kRow + (copy_dst ^ (S::kWords >= 8 ? ((j * S::kRowsPerCopy) & 7) * 16 : 0)); };
-        int page = -1, off16 = 0;
-        if (paged16) {
-            if (page_at - page_base == 32) {
-                page_base = page_at;
-                pages = pages_behind;
-                pages_behind = entry(in.b, page_base + 32 + lane);
-            }
-            page = __shfl_sync(0xffffffffu, pages, page_at - page_base);
-            off16 = page_off;
-            page_off += kBlock;
-            if (page_off == a.c.block_size) { page_off = 0; ++page_at; }
-            if (rows >= kBlock && (unsigned)page < page_limit) {                  // a whole block of a page
+        if (page_at - page_base >= 32) {
+            page_base += 32;
+            pages = pages_behind;
+            pages_behind = entry(in.b, page_base + 32 + lane);
+        }
+        const int at_page = page_at - page_base, off16 = page_off, passed = pages_in(off16 + kBlock);
+        page_at += passed;
+        page_off += kBlock - passed * page_size;
+        if (rows >= kBlock && off16 + kBlock <= page_size) {
+            const int page = __shfl_sync(0xffffffffu, pages, at_page);
+            if ((unsigned)page < page_limit) {                                    // a whole block of a page
                 const unsigned char* k_row = a.c.k + page * a.c.sb + off16 * a.c.st + in.head * a.c.sh + lane_from;
                 const unsigned char* v_row = k_row + v_less_k;
                 if (word_there) {
@@ -439,23 +438,14 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
                 return;
             }
         }
-        // a sequence's end, rows with pages of their own, pages that do not exist: row by row, zeros where there is none
-        const int r16 = lane & 15, token = token0 + r16;
+        // a sequence's end, blocks on several pages, pages that do not exist: row by row, zeros where there is none
+        const int r16 = lane & 15, row_page = pages_in(off16 + r16), which = at_page + row_page;
+        const int page_here = __shfl_sync(0xffffffffu, pages, which), page_there = __shfl_sync(0xffffffffu, pages_behind, which);     // (lane `which` % 32)
+        const int64_t p = which < 32 ? page_here : page_there, off = off16 + r16 - row_page * page_size;
         bool there = r16 < rows;
-        int64_t p = 0, off = 0;
-        if (there) {
-            if (paged16) {
-                p = page;
-                off = off16 + r16;
-            } else {
-                const int i = token / a.c.block_size;
-                off = token - (int64_t)i * a.c.block_size;
-                p = ld_dep(a.tables + (int64_t)in.b * a.ld_tables + i);
-            }
-            if (p < 0 || p >= a.c.num_blocks) {
-                there = false;
-                report_status(a.status, kDevBadPage);
-            }
+        if (there && (unsigned)p >= page_limit) {
+            there = false;
+            report_status(a.status, kDevBadPage);
         }
         const long long row_from = there ? p * a.c.sb + off * a.c.st + in.head * a.c.sh : -1;
 #pragma unroll 1
@@ -896,7 +886,10 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
     }
 
     // ---- segments that other CTAs have pieces of: the last one to come joins them --------------------------------------
+    // More than kJoin of them in two steps: first groups of about the square root of their number, each by the group's last CTA.  (One SM
+    // reads some 40 GB/s of pieces: 74 of 8 KB took it 15 us.)
     if ((open0 | open1) == 0) return;
+    auto group_of = [](int count) { return count <= kJoin ? count : (int)ceilf(sqrtf((float)count)); };
     __syncthreads();
     if (tid < 2) {
         bool last = false;
@@ -904,10 +897,12 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
             const Piece p = s_piece[__ffs(tid == 0 ? open0 : open1) - 1];
             const int c0 = apart ? blockIdx.x - own_part : (int)quotient(p.tile0, share);
             const int count = apart ? own_parts : (int)quotient(p.tile0 + p.tiles - 1, share) - c0 + 1;
+            const int size = group_of(count), first = ((int)blockIdx.x - c0) / size * size, members = min(size, count - first);
             s_cta0[tid] = c0;
             s_ctas[tid] = count;
-            last = arrive(a.counters + c0) == count - 1;
-            if (last) a.counters[c0] = 0;                                          // for the next call
+            int* const counter = a.counters + 2 * (c0 + first) + (first == 0);     // of the slot that the group's first piece is in
+            last = arrive(counter) == members - 1;
+            if (last) *counter = 0;                                                // for the next call
         }
         s_last[tid] = last;
     }
@@ -916,90 +911,93 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
     for (int w = 0; w < 2; ++w) {
         if (!s_last[w]) continue;
         const Piece p = s_piece[__ffs(w == 0 ? open0 : open1) - 1];
-        const int c0 = s_cta0[w], count = s_ctas[w];
+        const int c0 = s_cta0[w], count = s_ctas[w], size = group_of(count);
         // the first CTA's piece is its second one, the others' their first
-        const float* const piece0 = pieces + ((int64_t)c0 * 2 + 1) * kOut;
-        const float* const piece1 = pieces + ((int64_t)c0 * 2) * kOut;
+        float* const piece0 = pieces + ((int64_t)c0 * 2 + 1) * kOut;
+        float* const piece1 = pieces + ((int64_t)c0 * 2) * kOut;
         auto piece_of = [&](int i) { return i == 0 ? piece0 : piece1 + (uint32_t)i * (2 * kOut); };
-        // kSlices threads share a fragment's pieces, kAtOnce of them on their way at a time, the first beside the weights
+        // kSlices threads share a fragment's pieces
         constexpr int kSlices = S::kThreads > kUnits ? S::kThreads / kUnits : 1, kPerThread = kUnits > S::kThreads ? kUnits / S::kThreads : 1;
-        constexpr int kAtOnce = S::kThreads > 256 ? 10 : 20;
         const int slice = tid / kUnits;
-        uint4 raw[kAtOnce];
-        auto ask = [&](int unit, int i0) {
+        int start = ((int)blockIdx.x - c0) / size * size, stride = 1, n = min(size, count - start);
+#pragma unroll 1
+        for (;;) {
+            uint4 raw[kJoin / kSlices];
+            auto ask = [&](int unit) {
 #pragma unroll
-            for (int i = 0; i < kAtOnce; ++i)
-                if (i0 + i * kSlices < count) raw[i] = ld_dep_l2(reinterpret_cast<const uint4*>(piece_of(i0 + i * kSlices)) + unit);
-        };
-        bool asked = false;
-        for (int col = warp; col < kHeads; col += kWarps) {                        // a warp for a query head, a lane for a few CTAs
-            float pm[kMaxCtas / 32], pl[kMaxCtas / 32], top = kNone, sum = 0.f;
-#pragma unroll
-            for (int i = 0; i < kMaxCtas / 32; ++i) {
-                pm[i] = kNone;
-                pl[i] = 0.f;
-                if (i * 32 < count) {
-                    if (i * 32 + lane < count) {
-                        pm[i] = ld_dep_l2(piece_of(i * 32 + lane) + kPiece + col);
-                        pl[i] = ld_dep_l2(piece_of(i * 32 + lane) + kPiece + kHeads + col);
-                    }
+                for (int i = 0; i < kJoin / kSlices; ++i)
+                    if (slice + i * kSlices < n) raw[i] = ld_dep_l2(reinterpret_cast<const uint4*>(piece_of(start + (slice + i * kSlices) * stride)) + unit);
+            };
+            for (int col = warp; col < kHeads; col += kWarps) {                    // a warp for a query head, a lane for a piece
+                float pm = kNone, pl = 0.f;
+                if (lane < n) {
+                    pm = ld_dep_l2(piece_of(start + lane * stride) + kPiece + col);
+                    pl = ld_dep_l2(piece_of(start + lane * stride) + kPiece + kHeads + col);
                 }
+                const float top = warp_max(pm), f = exp2_approx(pm - top);
+                float sum = f * pl;
+                for (int x = 16; x; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+                if (lane < n) s_share[lane][col] = f;
+                if (lane == 0) { s_top[col] = top; s_sum[col] = sum; }
             }
-            if (!asked) ask(tid % kUnits, slice);
-            asked = true;
+            __syncthreads();
+            float4 v[kPerThread];
 #pragma unroll
-            for (int i = 0; i < kMaxCtas / 32; ++i) top = fmaxf(top, pm[i]);
-            top = warp_max(top);
+            for (int k = 0; k < kPerThread; ++k) {
+                const int unit = (tid + k * S::kThreads) % kUnits, col = (unit >> 5) % kN * 8 + 2 * t4;
+                v[k] = {0.f, 0.f, 0.f, 0.f};
+                ask(unit);
 #pragma unroll
-            for (int i = 0; i < kMaxCtas / 32; ++i) {
-                if (i * 32 < count) {
-                    const float f = exp2_approx(pm[i] - top);
-                    sum += f * pl[i];
-                    if (i * 32 + lane < count) s_share[i * 32 + lane][col] = f;
-                }
-            }
-            for (int x = 16; x; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
-            if (lane == 0) s_inv[col] = reciprocal(sum);
-        }
-        if (!asked) ask(tid % kUnits, slice);
-        __syncthreads();
-        float4 v[kPerThread];
-#pragma unroll
-        for (int k = 0; k < kPerThread; ++k) {
-            const int unit = (tid + k * S::kThreads) % kUnits, col = (unit >> 5) % kN * 8 + 2 * t4;
-            v[k] = {0.f, 0.f, 0.f, 0.f};
-            for (int i0 = slice; i0 < count; i0 += kAtOnce * kSlices) {
-                if (k > 0 || i0 != slice) ask(unit, i0);
-#pragma unroll
-                for (int i = 0; i < kAtOnce; ++i)
-                    if (i0 + i * kSlices < count) {
-                        const float2 f = *reinterpret_cast<const float2*>(&s_share[i0 + i * kSlices][col]);
+                for (int i = 0; i < kJoin / kSlices; ++i)
+                    if (slice + i * kSlices < n) {
+                        const float2 f = *reinterpret_cast<const float2*>(&s_share[slice + i * kSlices][col]);
                         v[k].x += f.x * __uint_as_float(raw[i].x); v[k].y += f.y * __uint_as_float(raw[i].y);
                         v[k].z += f.x * __uint_as_float(raw[i].z); v[k].w += f.y * __uint_as_float(raw[i].w);
                     }
             }
-        }
-        if (kSlices > 1) {
-            float4* const sums = reinterpret_cast<float4*>(ring);
-            if (slice > 0) sums[tid - kUnits] = v[0];
-            __syncthreads();
-            if (slice == 0) {
+            if (kSlices > 1) {
+                float4* const sums = reinterpret_cast<float4*>(ring);
+                if (slice > 0) sums[tid - kUnits] = v[0];
+                __syncthreads();
+                if (slice == 0) {
 #pragma unroll
-                for (int k = 1; k < kSlices; ++k) {
-                    const float4 y = sums[(k - 1) * kUnits + tid];
-                    v[0].x += y.x; v[0].y += y.y; v[0].z += y.z; v[0].w += y.w;
+                    for (int k = 1; k < kSlices; ++k) {
+                        const float4 y = sums[(k - 1) * kUnits + tid];
+                        v[0].x += y.x; v[0].y += y.y; v[0].z += y.z; v[0].w += y.w;
+                    }
                 }
             }
-        }
-        if (slice == 0) {
+            const bool all = size == count || stride > 1;
+            if (slice == 0) {
 #pragma unroll
-            for (int k = 0; k < kPerThread; ++k) {
-                const int frag = (tid + k * S::kThreads) >> 5, n = frag % kN;
-                result.store<kE4m3>(p.b, p.head0, p.heads, frag / kN, n, v[k],
-                                    *reinterpret_cast<const float2*>(&s_inv[n * 8 + 2 * t4]));
+                for (int k = 0; k < kPerThread; ++k) {
+                    const int unit = tid + k * S::kThreads, frag = unit >> 5, n8 = frag % kN, col = n8 * 8 + 2 * t4;
+                    const float2 top = *reinterpret_cast<const float2*>(&s_top[col]), sum = *reinterpret_cast<const float2*>(&s_sum[col]);
+                    if (all) {
+                        result.store<kE4m3>(p.b, p.head0, p.heads, frag / kN, n8, v[k], {reciprocal(sum.x), reciprocal(sum.y)});
+                    } else {                                                       // in place of the group's first
+                        float* const out = piece_of(start);
+                        reinterpret_cast<float4*>(out)[unit] = v[k];
+                        if (frag < kN && g == 0) {
+                            *reinterpret_cast<float2*>(out + kPiece + col) = top;
+                            *reinterpret_cast<float2*>(out + kPiece + kHeads + col) = sum;
+                        }
+                    }
+                }
             }
+            __syncthreads();                                                       // s_share and its companions are free again
+            if (all) break;
+            if (tid == 0) {
+                int* const counter = a.counters + 2 * kMaxCtas + c0;
+                s_again = arrive(counter) == (count + size - 1) / size - 1;
+                if (s_again) *counter = 0;
+            }
+            __syncthreads();
+            if (!s_again) break;
+            start = 0;
+            stride = size;
+            n = (count + size - 1) / size;
         }
-        __syncthreads();                                                           // s_share and s_inv are free again
     }
 }
 
