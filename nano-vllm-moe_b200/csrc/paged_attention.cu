@@ -48,6 +48,7 @@ struct Shape {
     static constexpr int kWarps = kWarps_;
     static constexpr int kStages = kStages_;
     static constexpr int kThreads = 32 * kWarps;
+    static constexpr int kJoinTiles = 8 / (kM * kN);                      // tiles that take a warp as long as a CTA's joining of a segment that others work on too
     static constexpr int kRow = kD * (kE4m3 ? 1 : 2);                     // bytes of a row
     static constexpr int kWords = kRow / 16;                              // 16-byte words of a row
     static constexpr int kRowsPerCopy = kWords >= 32 ? 1 : 32 / kWords;   // rows that a warp's copy instruction takes
@@ -203,7 +204,7 @@ template <class S>
 __global__ void __launch_bounds__(S::kThreads, 1)
 paged_attention_kernel(AttnArgs a, int group, int parts) {
     constexpr bool kE4m3 = S::kE4m3;
-    constexpr int kTile = S::kTile, kM = S::kM, kD = S::kD, kN = S::kN, kHeads = S::kHeads, kWarps = S::kWarps, kStages = S::kStages, kRow = S::kRow, kPiece = S::kPiece;
+    constexpr int kTile = S::kTile, kM = S::kM, kJoinTiles = S::kJoinTiles, kD = S::kD, kN = S::kN, kHeads = S::kHeads, kWarps = S::kWarps, kStages = S::kStages, kRow = S::kRow, kPiece = S::kPiece;
     extern __shared__ __align__(1024) unsigned char ring[];
     __shared__ Piece s_piece[2 * kWarps];
     // (read two heads at a time)
@@ -269,12 +270,12 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
         return f;
     };
     // Three ways to deal the list out.  (1) To CTAs that work on one segment each, some on the same, where no CTA's share grows much by that: joining
-    // the pieces of two segments takes a CTA twice as long.  Joining over CTAs costs as much as some eight tiles per warp, so where there is a CTA for every
+    // the pieces of two segments takes a CTA twice as long.  Joining over CTAs costs as much as kJoinTiles per warp, so where there is a CTA for every
     // segment and none is that much longer than an even share, each has one.  (2) Short segments: in even shares, rounded to whole segments.
     // (3) In even shares.
     const int longest = __reduce_max_sync(0xffffffffu, lane_most), grid = (int)gridDim.x;
     const bool few = a.batch <= grid && a.batch * segments <= grid;
-    bool apart = few && longest <= 9 * kWarps;                                    // (a share is a tile per warp at least)
+    bool apart = few && longest <= (1 + kJoinTiles) * kWarps;                                    // (a share is a tile per warp at least)
     int64_t total = 0, before = 0, share = kWarps, cta0, cta1;                    // this CTA's places: of the list, or (apart) of one segment's part of it
     Found own = {};                                                               // apart: that segment
     int own_segment = 0, own_part = 0, own_parts = 1;                             // ... which of its CTAs this is, and of how many
@@ -293,7 +294,7 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
         share = quotient(total + grid - 1, grid);
         if (share < kWarps) share = kWarps;
         if (few) {
-            const int64_t cta_share = longest <= share + 8 * kWarps ? longest : share + share / 16;
+            const int64_t cta_share = longest <= share + kJoinTiles * kWarps ? longest : share + share / 16;
             auto units_of = [&](int len) { return quotient(tiles_of(len) + cta_share - 1, cta_share) * segments; };      // CTAs of a sequence
             int64_t units = 0;
             if (stretch == 1) units = lane < a.batch ? units_of(lane_len) : 0;
@@ -316,7 +317,7 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
             cta0 = blockIdx.x * share;
             cta1 = cta0 + share < total ? cta0 + share : total;
             if (cta0 >= total) return;
-            if (longest <= 2 * kWarps) {                                          // ... to the nearer end of a segment
+            if (longest <= kJoinTiles / 4 * kWarps) {                             // ... to the nearer end of a segment
 #pragma unroll 1
                 for (int side = 0; side < 2; ++side) {
                     const int64_t place = side == 0 ? cta0 : cta1;
@@ -1030,7 +1031,8 @@ cudaError_t launch(const AttnArgs& a, int group, int parts, cudaStream_t stream)
 // more than 8 (256 channels: 8, whose sums fill the registers), the rest of a larger group as segments of their own.
 template <class F>
 auto with_shape(bool e4m3, int64_t dim, int64_t group, F&& f) {
-    const bool wide = group > 8;
+    // (16 at a time take a warp 1.5 us for 16 tokens of an e4m3 cache, 8 at a time 1.6 us for 32; so an odd number of eights goes one by one)
+    const bool wide = group > 8 && (!e4m3 || (group + 7) / 8 % 2 == 0);
     if (e4m3) {
         if (dim <= 64) return wide ? f(Shape<true, 64, 2, 1, 8, 6>()) : f(Shape<true, 64, 1, 2, 16, 3>());
         if (dim <= 128) return wide ? f(Shape<true, 128, 2, 1, 8, 6>()) : f(Shape<true, 128, 1, 2, 8, 3>());
