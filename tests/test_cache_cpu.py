@@ -69,6 +69,7 @@ def test_bad_arguments_are_refused(pkg, memory):
     def attend(q=p, qr=128, qh=32, tables=p, ld=4, pages=4, lens=p, batch=2, heads=4, out_scale=None, out=p, ld_out=128, ws=p, size=need):
         return lib.fp8lin_paged_attention(c, q, qr, qh, tables, ld, pages, lens, batch, heads, 1.0, out_scale, out, ld_out, ws, size, None)
     assert attend(batch=0, q=None) == L.OK
+    assert attend(batch=1 << 24, heads=256, qr=128 * 256) == L.ERR_SHAPE
     assert attend(heads=3) == attend(heads=0) == attend(batch=-1) == attend(ld=3) == L.ERR_SHAPE
     assert attend(q=None) == attend(tables=None) == attend(lens=None) == attend(out=None) == L.ERR_NULL
     assert attend(q=p + 2) == attend(qr=100) == attend(qh=12) == attend(out=p + 8) == attend(ld_out=120) == attend(ld_out=132) == L.ERR_ALIGN
@@ -120,3 +121,31 @@ def test_cache_layout(pkg, dtype):
         assert c.k_scale.shape == (3, 8, 2) and c.k_scale.stride() == (16, 1, 8)
     else:
         assert c.k_scale is None and c.v_scale is None
+
+
+def test_row_parallel_sums_what_codes_give(pkg, monkeypatch):
+    """Codes of a decode step through o_proj on several ranks: the local product, summed by the all-reduce."""
+    from importlib import import_module
+    linear = import_module("nano-vllm-moe_b200.layers.linear")
+    seen = []
+
+    class Method(pkg.QuantizeMethodBase):
+        def create_weights(self, layer, **kw):
+            pass
+
+        def apply(self, layer, x, bias=None):
+            seen.append((x, bias))
+            return torch.ones(2, 8)
+
+        def process_weights_after_loading(self, layer):
+            pass
+    lay = pkg.RowParallelLinear(32, 8, quant_method=Method())
+    lay.tp_size, lay.tp_rank = 2, 1
+    monkeypatch.setattr(linear.dist, "all_reduce", lambda y, group=None: y.mul_(2))
+    codes = pkg.QuantizedActivation(torch.zeros(2, 16, dtype=torch.uint8), torch.tensor(1.0))
+    assert torch.equal(lay(codes), torch.full((2, 8), 2.0)) and seen == [(codes, None)]
+    lay.reduce_results = False
+    assert torch.equal(lay(codes), torch.ones(2, 8))
+    lay.reduce_results = "scatter"
+    with pytest.raises(ValueError, match="codes"):
+        lay(codes)

@@ -153,6 +153,54 @@ def test_many_sequences(e4m3):
 
 
 @pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("seed", range(12))
+def test_batches_of_any_lengths(seed, e4m3):
+    """Lengths spread over their logarithm, so that sequences of all sizes share warps and CTAs in all ways; heads and pages at random."""
+    r = np.random.default_rng(seed)
+    heads, kv_heads, dim = [(28, 4, 128), (14, 2, 64), (16, 16, 128), (20, 1, 128), (12, 12, 64), (24, 2, 96), (8, 1, 256), (32, 8, 128)][seed % 8]
+    batch = int(r.choice([1, 2, 5, 17, 33, 70, 150]))
+    longest = int(r.choice([40, 400, 4000]) * (1 if batch > 30 else 4))
+    lengths = [int(n) for n in np.exp(r.uniform(0, math.log(longest), batch))]
+    for i in range(0, batch, 7):
+        lengths[i] = 0
+    check(Cache(lengths, kv_heads, dim, int(r.choice([3, 8, 16, 24, 64, 256])), e4m3, seed=seed), queries(batch, heads, dim, seed=seed))
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("heads, kv_heads, length", [(8, 1, 70000), (20, 1, 33333), (16, 16, 9000), (3, 3, 30000)])
+def test_one_sequence_over_many_ctas(heads, kv_heads, length, e4m3):
+    """From a few pieces of a head to so many that they are joined in two steps."""
+    c, q = Cache([length], kv_heads, 128, 64, e4m3, seed=7), queries(1, heads, 128, spread=2.0)
+    first = check(c, q)
+    for _ in range(3):
+        assert torch.equal(kernels().paged_attention(q, *c.args(), **c.scales()), first)
+
+
+def test_codes_as_bytes_and_heads_apart():
+    """A cache of uint8 codes is one of float8; queries whose heads do not follow one another."""
+    c = Cache([100, 37], 2, 64, 16, True)
+    wide = torch.randn(2, 6, 3, 64, device="cuda").to(torch.bfloat16)
+    q = wide[:, :, 1]
+    want = check(c, q)
+    k, v = c.k.view(torch.uint8), c.v.view(torch.uint8)
+    assert torch.equal(kernels().paged_attention(q, k, v, c.tables, c.lens, **c.scales()), want)
+    cu = torch.tensor([0, 100, 137], dtype=torch.int32, device="cuda")
+    for x, y in zip(kernels().kv_cache_read(k, v, c.tables, cu, 137, c.ks, c.vs), kernels().kv_cache_read(c.k, c.v, c.tables, cu, 137, c.ks, c.vs)):
+        assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+def test_sequences_that_share_pages(e4m3):
+    """A common beginning in the same pages, as of a shared prompt."""
+    c = Cache([200, 200], 2, 64, 16, e4m3, seed=8)
+    tables = c.tables.clone()
+    tables[1, :6] = tables[0, :6]
+    q = queries(2, 8, 64)
+    c.tables, c.rows[1] = tables, [torch.cat([a[:96], b[96:]]) for a, b in zip(c.rows[0], c.rows[1])]
+    check(c, q)
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
 def test_empty_batch_and_all_empty(e4m3):
     assert kernels().paged_attention(queries(0, 14, 64), *Cache([], 2, 64, 16, e4m3).args(), **Cache([], 2, 64, 16, e4m3).scales()).shape == (0, 14, 64)
     c = Cache([0] * 40, 2, 64, 16, e4m3)
@@ -308,6 +356,30 @@ def test_write_and_read_back(pkg, tokens, kv_heads, dim, block, e4m3):
     for out, cache, scale in zip(got, (c.k, c.v), (c.k_scale, c.v_scale)):
         flat = (cache.float() * scale[..., None] if e4m3 else cache).to(torch.bfloat16).reshape(blocks * block, kv_heads, dim)
         assert torch.equal(out, torch.cat([flat[:ends[1]], flat[:ends[3] - ends[2]]]))
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("tokens, kv_heads, dim", [(5000, 4, 128), (3001, 3, 80), (700, 40, 64), (2000, 1, 256), (9000, 2, 48), (150, 130, 16)])
+def test_many_rows_there_and_back(pkg, tokens, kv_heads, dim, e4m3):
+    """More than a block's turn, heads that divide it and heads that do not; the formula's codes byte for byte, and many sequences."""
+    k, v = rows_of(tokens, kv_heads, dim, seed=dim)
+    block = 16
+    c = pkg.PagedKVCache(-(-tokens // block), block, kv_heads, dim, E4M3 if e4m3 else torch.bfloat16)
+    slots = torch.randperm(c.k.shape[0] * block, generator=torch.Generator().manual_seed(1))[:tokens].cuda()
+    c.write(k, v, slots.to(torch.int32))
+    ends = sorted(np.random.default_rng(2).integers(0, 3000, 1500).tolist())          # (more than a block keeps at hand)
+    ends = [0] + [min(e, 3 * block) for e in ends[:3]] + [3 * block + i // 8 for i in range(1500)]
+    tables = torch.arange(c.k.shape[0], dtype=torch.int32, device="cuda").expand(len(ends) - 1, -1).contiguous()
+    got = c.read(tables, torch.tensor(ends, dtype=torch.int32, device="cuda"), ends[-1])
+    for x, cache, scale, out in ((k, c.k, c.k_scale, got[0]), (v, c.v, c.v_scale, got[1])):
+        at = slots // block, slots % block
+        if e4m3:
+            codes, s = quantised(x)
+            assert torch.equal(cache.view(torch.uint8)[at], codes.view(torch.uint8)) and torch.equal(scale[at], s)
+        else:
+            assert torch.equal(cache[at], x)
+        flat = (cache.float() * scale[..., None] if e4m3 else cache).to(torch.bfloat16).reshape(-1, kv_heads, dim)
+        assert torch.equal(out, torch.cat([flat[:b - a] for a, b in zip(ends, ends[1:])]))
 
 
 @pytest.mark.parametrize("order", ["heads", "tokens", "wide"])
