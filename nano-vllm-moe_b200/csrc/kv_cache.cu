@@ -13,8 +13,12 @@
 // holds 16, even lanes in the row's first half and odd ones in its second, and neighbours exchange half of theirs on the way.
 // (Reading 206 MB back took 46 us with a lane's 16 channels side by side on both sides, which writes half sectors, and 50 with two
 // times eight codes a lane.)
-// A thread has kDeep rows in flight: four, or one where the call has no more for it (2.3 instead of 3.4 us for 64 tokens of 4 heads).  A block takes a few tokens at a time with all their heads, keys and values; what a token needs (its slot; its
-// sequence, page and offset) is looked up once, a turn early: looked up when it was needed, it took longer than the rows.
+// A thread has kDeep rows in flight: four, or one where the call has no more for it (2.3 instead of 3.4 us for 64 tokens of 4 heads).
+// A block takes a few tokens at a time with all their heads, keys and values; what a token needs (its slot; its sequence, page and
+// offset) is looked up once, a turn early: looked up when it was needed, it took longer than the rows.
+//
+// Measured (B200, in a row of calls, inputs larger than L2): writing 51 MB (16384 tokens of 4 heads of 128, to codes) 14.9 us, 17 MB
+// 3.8; reading 206 MB of codes back 41 us, 5.0 TB/s, 134 MB of bf16 24 us, 5.6 TB/s.  A kernel that only copies 34 MB takes 8.5 us.
 #include "common.cuh"
 #include "kernels.h"
 
@@ -340,7 +344,8 @@ static cudaError_t launch_cache(Kernel kernel, int blocks, cudaStream_t stream, 
 cudaError_t launch_kv_cache_write(const CacheView& c, const CacheRows& x, const int* slots, int* status, cudaStream_t stream) {
     const bool few = few_rows(c, x.rows);
     const CacheGrid g = cache_grid(c, x.rows, few ? 1 : 4);
-    auto kernel = c.e4m3 ? (few ? kv_cache_write_kernel<true, 1> : kv_cache_write_kernel<true, 4>) : (few ? kv_cache_write_kernel<false, 1> : kv_cache_write_kernel<false, 4>);
+    auto kernel = c.e4m3 ? (few ? kv_cache_write_kernel<true, 1> : kv_cache_write_kernel<true, 4>)
+                         : (few ? kv_cache_write_kernel<false, 1> : kv_cache_write_kernel<false, 4>);
     return launch_cache(kernel, g.blocks, stream, c, x, slots, g, status);
 }
 
@@ -348,7 +353,8 @@ cudaError_t launch_kv_cache_read(const CacheView& c, const CacheRows& y, const i
                                  int64_t batch, int* status, cudaStream_t stream) {
     const bool few = few_rows(c, y.rows);
     const CacheGrid g = cache_grid(c, y.rows, few ? 1 : 4);
-    auto kernel = c.e4m3 ? (few ? kv_cache_read_kernel<true, 1> : kv_cache_read_kernel<true, 4>) : (few ? kv_cache_read_kernel<false, 1> : kv_cache_read_kernel<false, 4>);
+    auto kernel = c.e4m3 ? (few ? kv_cache_read_kernel<true, 1> : kv_cache_read_kernel<true, 4>)
+                         : (few ? kv_cache_read_kernel<false, 1> : kv_cache_read_kernel<false, 4>);
     return launch_cache(kernel, g.blocks, stream, c, y, tables, ld_tables, max_pages, cu_seqlens, (int)batch, g, status);
 }
 

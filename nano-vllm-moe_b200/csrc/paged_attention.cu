@@ -174,30 +174,41 @@ struct Result {
     const AttnArgs& a;
     const ExactDiv div;
     __device__ __forceinline__ explicit Result(const AttnArgs& args) : a(args), div(args.out_scale ? fmaxf(ld_dep(args.out_scale), 1e-12f) : 1.f) {}
-    // channels d and d + 1 of a query head
-    __device__ __forceinline__ void store2(int b, int head, int d, uint32_t w) const {
-        const int64_t at = (int64_t)b * a.ld_out + (int64_t)head * a.c.dim + d;
-        if (a.out_scale) *reinterpret_cast<uint16_t*>(static_cast<unsigned char*>(a.out) + at) = cvt_e4m3x2(div(bf16_lo(w)), div(bf16_hi(w)));
+    // two channels of a query head, from element `at` of the result on
+    template <bool kCodes>
+    __device__ __forceinline__ void put(int64_t at, uint32_t w) const {
+        if (kCodes) *reinterpret_cast<uint16_t*>(static_cast<unsigned char*>(a.out) + at) = cvt_e4m3x2(div(bf16_lo(w)), div(bf16_hi(w)));
         else *reinterpret_cast<uint32_t*>(static_cast<__nv_bfloat16*>(a.out) + at) = w;
     }
-    // A fragment of the sums O^T of 16 channels from c * 16 on and of query heads n * 8 + 2 t4 (x, z) and n * 8 + 2 t4 + 1 (y, w),
-    // times those heads' `inv`.  All lanes of a warp together.
-    template <bool kE4m3>
-    __device__ __forceinline__ void store(int b, int head0, int heads, int c, int n, float4 v, float2 inv) const {
-        const int g = (threadIdx.x & 31) >> 2, t4 = threadIdx.x & 3;
-        if (c * 16 >= a.c.dim) return;
-        if (kE4m3) {                                                              // rows g and g + 8: channels 2g and 2g + 1
-            const int col = n * 8 + 2 * t4;
-            if (col < heads) store2(b, head0 + col, c * 16 + 2 * g, pack_bf16x2(v.x * inv.x, v.z * inv.x));
-            if (col + 1 < heads) store2(b, head0 + col + 1, c * 16 + 2 * g, pack_bf16x2(v.y * inv.y, v.w * inv.y));
-        } else {                                                                  // channels g and g + 8: transposed, a lane has two of head g
-            const uint32_t lo = transposed(pack_bf16x2(v.x * inv.x, v.y * inv.y)), hi = transposed(pack_bf16x2(v.z * inv.x, v.w * inv.y));
-            const int col = n * 8 + g;
-            if (col < heads) {
-                store2(b, head0 + col, c * 16 + 2 * t4, lo);
-                store2(b, head0 + col, c * 16 + 8 + 2 * t4, hi);
+    // kCount fragments of the sums O^T, of 16 channels each from c * 16 on, and of query heads n * 8 + 2 t4 (x, z) and
+    // n * 8 + 2 t4 + 1 (y, w), times those heads' `inv`.  All lanes of a warp together.
+    template <bool kE4m3, bool kCodes, int kCount, class Fragment>
+    __device__ __forceinline__ void store(int b, int head0, int heads, int c, int n, Fragment fragment, float2 inv) const {
+        const int g = (threadIdx.x & 31) >> 2, t4 = threadIdx.x & 3, dim = a.c.dim;
+        const int col = n * 8 + (kE4m3 ? 2 * t4 : g);
+        // e4m3: rows g and g + 8 of a fragment are channels 2g and 2g + 1; bf16: g and g + 8, and transposed a lane has two of head g
+        const int64_t at = (int64_t)b * a.ld_out + (int64_t)(head0 + col) * dim + c * 16 + 2 * (kE4m3 ? g : t4);
+        const bool first = col < heads, second = kE4m3 ? col + 1 < heads : first;
+#pragma unroll
+        for (int i = 0; i < kCount; ++i) {
+            if ((c + i) * 16 >= dim) break;
+            const float4 v = fragment(i);
+            uint32_t x, y;
+            if (kE4m3) {
+                x = pack_bf16x2(v.x * inv.x, v.z * inv.x);
+                y = pack_bf16x2(v.y * inv.y, v.w * inv.y);
+            } else {
+                x = transposed(pack_bf16x2(v.x * inv.x, v.y * inv.y));
+                y = transposed(pack_bf16x2(v.z * inv.x, v.w * inv.y));
             }
+            if (first) put<kCodes>(at + i * 16, x);
+            if (second) put<kCodes>(at + i * 16 + (kE4m3 ? dim : 8), y);
         }
+    }
+    template <bool kE4m3, int kCount, class Fragment>
+    __device__ __forceinline__ void store(int b, int head0, int heads, int c, int n, Fragment fragment, float2 inv) const {
+        if (a.out_scale) store<kE4m3, true, kCount>(b, head0, heads, c, n, fragment, inv);
+        else store<kE4m3, false, kCount>(b, head0, heads, c, n, fragment, inv);
     }
 };
 
@@ -211,7 +222,8 @@ template <class S>
 __global__ void __launch_bounds__(S::kThreads, 1)
 paged_attention_kernel(AttnArgs a, int group, int parts) {
     constexpr bool kE4m3 = S::kE4m3;
-    constexpr int kTile = S::kTile, kM = S::kM, kJoinTiles = S::kJoinTiles, kD = S::kD, kN = S::kN, kHeads = S::kHeads, kWarps = S::kWarps, kStages = S::kStages, kRow = S::kRow, kPiece = S::kPiece;
+    constexpr int kTile = S::kTile, kM = S::kM, kJoinTiles = S::kJoinTiles, kD = S::kD, kN = S::kN, kHeads = S::kHeads;
+    constexpr int kWarps = S::kWarps, kStages = S::kStages, kRow = S::kRow, kPiece = S::kPiece;
     extern __shared__ __align__(1024) unsigned char ring[];
     __shared__ Piece s_piece[2 * kWarps];
     // (read two heads at a time)
@@ -350,7 +362,8 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
     const uint32_t my_ring_at = smem_addr(my_ring);
     const int row_bytes = a.c.dim * (kE4m3 ? 1 : 2);
     const int page_size = a.c.block_size, page_magic = page_size <= kBlock ? 65536 / page_size + 1 : 0;
-    auto pages_in = [&](int tokens) { return page_size > kBlock ? (tokens >= page_size ? 1 : 0) : tokens * page_magic >> 16; };      // up to 30 tokens, or less than two pages
+    // (of up to 30 tokens, or of less than two pages)
+    auto pages_in = [&](int tokens) { return page_size > kBlock ? (tokens >= page_size ? 1 : 0) : tokens * page_magic >> 16; };
     const int g = lane >> 2, t4 = lane & 3;
     if (row_bytes < kRow) {                                         // channels behind head_dim: zeros once, they are never copied to
         for (int i = lane * 16; i < kStages * S::kStageBytes; i += 512) *reinterpret_cast<uint4*>(my_ring + i) = {0, 0, 0, 0};
@@ -801,10 +814,13 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
 #pragma unroll
                 for (int n = 0; n < kN; ++n) {
                     const float2 inv = at.len > 0 ? float2{reciprocal(l[n][0]), reciprocal(l[n][1])} : float2{0.f, 0.f};
+                    // A copy of the loop for bf16 and one for codes take less time than a branch in it (8 x 2048 tokens 16.2 -> 15.5 us, 256 x 512 13.7 ->
+                    // 13.3), except where two blocks of e4m3 tokens a turn leave no registers for it (131071 tokens 34.4 -> 35.8)
+                    constexpr int kAtOnce = kE4m3 && kM == 2 ? 1 : kD / 16;
 #pragma unroll
-                    for (int c = 0; c < kD / 16; ++c)
-                        result.store<kE4m3>(at.b, at.head * group + at.part * kHeads, min(kHeads, group - at.part * kHeads), c, n,
-                                            {o[c][n][0], o[c][n][1], o[c][n][2], o[c][n][3]}, inv);
+                    for (int c = 0; c < kD / 16; c += kAtOnce)
+                        result.store<kE4m3, kAtOnce>(at.b, at.head * group + at.part * kHeads, min(kHeads, group - at.part * kHeads), c, n,
+                                                     [&](int i) { return float4{o[c + i][n][0], o[c + i][n][1], o[c + i][n][2], o[c + i][n][3]}; }, inv);
                 }
             } else {
                 if (lane == 0)
@@ -891,7 +907,7 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
             }
         } else {
             const Piece p = s_piece[at_first];
-            result.store<kE4m3>(p.b, p.head0, p.heads, frag / kN, n, v, {reciprocal(sum.x), reciprocal(sum.y)});
+            result.store<kE4m3, 1>(p.b, p.head0, p.heads, frag / kN, n, [&](int) { return v; }, {reciprocal(sum.x), reciprocal(sum.y)});
         }
     }
 
@@ -984,7 +1000,7 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
                     const int unit = tid + k * S::kThreads, frag = unit >> 5, n8 = frag % kN, col = n8 * 8 + 2 * t4;
                     const float2 top = *reinterpret_cast<const float2*>(&s_top[col]), sum = *reinterpret_cast<const float2*>(&s_sum[col]);
                     if (all) {
-                        result.store<kE4m3>(p.b, p.head0, p.heads, frag / kN, n8, v[k], {reciprocal(sum.x), reciprocal(sum.y)});
+                        result.store<kE4m3, 1>(p.b, p.head0, p.heads, frag / kN, n8, [&](int) { return v[k]; }, {reciprocal(sum.x), reciprocal(sum.y)});
                     } else {                                                       // in place of the group's first
                         float* const out = piece_of(start);
                         reinterpret_cast<float4*>(out)[unit] = v[k];

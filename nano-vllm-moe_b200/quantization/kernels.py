@@ -323,7 +323,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     sequence b: ``softmax(scale * q . K^T) V``, bfloat16 [B, heads, head_dim].  q: bfloat16 [B, heads, head_dim], any strides of whole 16-byte
     words; ``heads`` a multiple of the cache's kv_heads; ``scale`` None: 1 / sqrt(head_dim).  A context of 0 gives zeros.
     With ``out_scale`` (one float32 on the device, the input scale of the linear behind the attention) the result is the uint8
-    e4m3 codes that ``quantize_activation`` makes of the bfloat16 one.  ``out``: [B, heads, head_dim] or [B, heads * head_dim]."""
+    e4m3 codes that ``quantize_activation`` makes of the bfloat16 one.  ``out``: [B, heads, head_dim] or [B, heads * head_dim]; a bfloat16
+    result may go to ``q`` itself, where its heads lie one behind the other."""
     return _lib.host().paged_attention(q, k_cache, v_cache, block_tables, context_lens, scale, k_scale, v_scale, out_scale, out)
 
 

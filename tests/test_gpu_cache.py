@@ -284,6 +284,20 @@ def test_outputs_of_the_caller():
 
 
 @pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("lengths", [[7], [5000], [1, 0, 300, 17, 2000, 64], [40 + 7 * i for i in range(200)]], ids=len)
+def test_result_in_place_of_the_queries(lengths, e4m3):
+    """Every reader of a query has read it when its result is there: the same bits as in memory of its own."""
+    heads, kv_heads, dim = 24, 2, 128
+    c = Cache(lengths, kv_heads, dim, 16, e4m3)
+    q = queries(len(lengths), heads, dim)
+    want = kernels().paged_attention(q, *c.args(), **c.scales())
+    for _ in range(5):
+        own = queries(len(lengths), heads, dim)
+        assert kernels().paged_attention(own, *c.args(), out=own, **c.scales()).data_ptr() == own.data_ptr()
+        assert torch.equal(own, want)
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
 def test_offsets_beyond_32_bits(e4m3):
     """The last pages of a cache of more than 4 GB."""
     dim, heads, block = 128, 4, 256
