@@ -18,7 +18,9 @@
 // offset) is looked up once, a turn early: looked up when it was needed, it took longer than the rows.
 //
 // Measured (B200, in a row of calls, inputs larger than L2): writing 51 MB (16384 tokens of 4 heads of 128, to codes) 14.9 us, 17 MB
-// 3.8; reading 206 MB of codes back 41 us, 5.0 TB/s, 134 MB of bf16 24 us, 5.6 TB/s.  A kernel that only copies 34 MB takes 8.5 us.
+// 3.8; reading 206 MB of codes back 39 us, 5.3 TB/s, 134 MB of bf16 24 us, 5.5 TB/s.  A kernel that only copies 34 MB takes 8.5 us.
+#include <algorithm>
+
 #include "common.cuh"
 #include "kernels.h"
 
@@ -26,7 +28,8 @@ namespace fp8lin {
 
 constexpr int kCacheThreads = 256;
 constexpr int kMaxTokens = 64;        // tokens of a block's turn
-constexpr int kCacheBlocks = 8;       // blocks of a launch per SM, twice what it holds at a time
+constexpr int kCacheBlocks = 8;       // blocks of a launch per SM, twice what it holds
+constexpr int kHeld = 4;              // blocks that an SM holds at a time, of threads with four rows in flight
 constexpr int kMaxEnds = 1024;        // sequences whose ends fit a block's shared memory
 
 struct CacheGrid {
@@ -243,7 +246,7 @@ kv_cache_read_kernel(CacheView c, CacheRows y, const int* tables, int64_t ld_tab
             at = b < 0 ? 0 : row - ld_dep(cu + b);
         }
         if (b < 0) return l;
-        const int64_t i = at / c.block_size;
+        const int64_t i = (uint32_t)at / (uint32_t)c.block_size;              // (a division of 64 bits is a hundred instructions, every turn)
         l.off = at - i * c.block_size;
         l.there = true;
         if (i < max_pages) l.page = ld_dep(tables + b * ld_tables + i);
@@ -312,14 +315,34 @@ kv_cache_read_kernel(CacheView c, CacheRows y, const int* tables, int64_t ld_tab
     }
 }
 
-// Tokens of a block's turn: as many as its threads take at once, `deep` rows each; fewer where that would leave SMs without a block.
+// Tokens of a block's turn: an SM's share where that is less than what a block's threads take at once, `deep` rows each.  Else that many, or
+// the power of two below, or twice as many where all blocks that the chip holds still get a turn, whichever leaves the SM with the most turns
+// the least to do.  A turn costs, in terms of the bytes of what the threads take at once, those of its tokens, one for each step of its threads and
+// a quarter beside them.  (Reading up to 1404 tokens of 10 heads of 80 for 11 sequences: 6 or 12 tokens 21.5 us, the power of two 28.2; 206 MB of 8
+// heads: 16 tokens 38.8, 8 tokens 40.9; writing 16842 tokens of 2 heads of 128: 32 tokens 7.5, 64, too few for the chip's blocks, 11.2.)
 static CacheGrid cache_grid(const CacheView& c, int64_t rows, int deep) {
     CacheGrid g = {1, 1, 0, 0};
     while ((16 << g.lanes_log2) < c.dim) ++g.lanes_log2;
-    const int at_once = (kCacheThreads >> g.lanes_log2) * deep / (2 * c.kv_heads);
-    while (g.tokens < kMaxTokens && 2 * g.tokens <= at_once && rows > (int64_t)g.tokens * sm_count()) g.tokens *= 2;
+    const int at_once = std::min((kCacheThreads >> g.lanes_log2) * deep / (2 * c.kv_heads), kMaxTokens);
+    const int64_t sms = sm_count(), spread = (rows + sms - 1) / sms;
+    if (spread <= at_once) {
+        g.tokens = (int)spread;
+    } else if (at_once > 1) {
+        int64_t least = INT64_MAX;
+        auto consider = [&](int tokens, int steps) {
+            const int64_t cost = ((rows + tokens * sms - 1) / (tokens * sms)) * (4 * tokens + (4 * steps + 1) * at_once);
+            if (tokens > kMaxTokens || cost > least) return;
+            least = cost;
+            g.tokens = tokens;
+        };
+        int power = 1;
+        while (2 * power <= at_once) power *= 2;
+        consider(power, 1);
+        consider(at_once, 1);
+        if (rows >= 2 * at_once * sms * kHeld) consider(2 * at_once, 2);
+    }
     g.turns = (rows + g.tokens - 1) / g.tokens;
-    const int64_t most = (int64_t)kCacheBlocks * sm_count();
+    const int64_t most = kCacheBlocks * sms;
     g.blocks = (int)(g.turns < most ? g.turns : most);
     return g;
 }
