@@ -373,7 +373,7 @@ def test_write_and_read_back(pkg, tokens, kv_heads, dim, block, e4m3):
 
 
 @pytest.mark.parametrize("e4m3", [False, True])
-@pytest.mark.parametrize("tokens, kv_heads, dim", [(5000, 4, 128), (3001, 3, 80), (700, 40, 64), (2000, 1, 256), (9000, 2, 48), (150, 130, 16)])
+@pytest.mark.parametrize("tokens, kv_heads, dim", [(5000, 4, 128), (3001, 3, 80), (700, 40, 64), (2000, 1, 256), (9000, 2, 48), (150, 130, 16), (20000, 10, 80), (9999, 16, 128)])
 def test_many_rows_there_and_back(pkg, tokens, kv_heads, dim, e4m3):
     """More than a block's turn, heads that divide it and heads that do not; the formula's codes byte for byte, and many sequences."""
     k, v = rows_of(tokens, kv_heads, dim, seed=dim)
@@ -394,6 +394,25 @@ def test_many_rows_there_and_back(pkg, tokens, kv_heads, dim, e4m3):
             assert torch.equal(cache[at], x)
         flat = (cache.float() * scale[..., None] if e4m3 else cache).to(torch.bfloat16).reshape(-1, kv_heads, dim)
         assert torch.equal(out, torch.cat([flat[:b - a] for a, b in zip(ends, ends[1:])]))
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("kv_heads, dim", [(10, 80), (16, 128), (1, 16)])
+def test_reads_of_every_length(pkg, kv_heads, dim, e4m3):
+    """From one token to more than the chip's blocks hold at a time; what lies behind the last sequence stays as it was."""
+    block, blocks = 24, 1600
+    c = pkg.PagedKVCache(blocks, block, kv_heads, dim, E4M3 if e4m3 else torch.bfloat16)
+    c.write(*rows_of(blocks * block, kv_heads, dim, seed=4), torch.arange(blocks * block, dtype=torch.int32, device="cuda"))
+    pages = torch.randperm(blocks, generator=torch.Generator().manual_seed(5)).cuda()
+    tables = torch.stack([pages[:800], pages[800:]]).to(torch.int32)
+    for ends in ([0, 1, 1], [0, 700, 1000], [0, 5, 9001], [0, 19199, 30011], [0, 0, 7111]):
+        rows = ends[-1] + 3
+        out = [torch.full((rows, kv_heads, dim), 7.0, dtype=torch.bfloat16, device="cuda") for _ in "kv"]
+        kernels().kv_cache_read(c.k, c.v, tables, torch.tensor(ends, dtype=torch.int32, device="cuda"), rows, c.k_scale, c.v_scale, *out)
+        for cache, scale, got in ((c.k, c.k_scale, out[0]), (c.v, c.v_scale, out[1])):
+            flat = (cache.float() * scale[..., None] if e4m3 else cache).to(torch.bfloat16)
+            want = [flat[tables[b].long()].reshape(-1, kv_heads, dim)[:ends[b + 1] - ends[b]] for b in range(2)]
+            assert torch.equal(got, torch.cat([*want, torch.full_like(got[:3], 7.0)]))
 
 
 @pytest.mark.parametrize("order", ["heads", "tokens", "wide"])
