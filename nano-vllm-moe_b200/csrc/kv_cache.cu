@@ -318,8 +318,8 @@ kv_cache_read_kernel(CacheView c, CacheRows y, const int* tables, int64_t ld_tab
 // Tokens of a block's turn: an SM's share where that is less than what a block's threads take at once, `deep` rows each.  Else that many, or
 // the power of two below, or twice as many where all blocks that the chip holds still get a turn, whichever leaves the SM with the most turns
 // the least to do.  A turn costs, in terms of the bytes of what the threads take at once, those of its tokens, one for each step of its threads and
-// a quarter beside them.  (Reading up to 1404 tokens of 10 heads of 80 for 11 sequences: 6 or 12 tokens 21.5 us, the power of two 28.2; 206 MB of 8
-// heads: 16 tokens 38.8, 8 tokens 40.9; writing 16842 tokens of 2 heads of 128: 32 tokens 7.5, 64, too few for the chip's blocks, 11.2.)
+// a quarter beside them.  (Reading up to 1404 tokens of 10 heads of 80 for 11 sequences: 6 or 12 tokens 21.5 us, the power of two 28.2; 206 MB of 4
+// heads of 128: 32 tokens 38.8, 16 tokens 40.9; writing 16842 tokens of 2 heads of 128: 32 tokens 7.5, 64, too few for the chip's blocks, 11.2.)
 static CacheGrid cache_grid(const CacheView& c, int64_t rows, int deep) {
     CacheGrid g = {1, 1, 0, 0};
     while ((16 << g.lanes_log2) < c.dim) ++g.lanes_log2;

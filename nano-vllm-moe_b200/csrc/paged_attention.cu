@@ -814,8 +814,8 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
 #pragma unroll
                 for (int n = 0; n < kN; ++n) {
                     const float2 inv = at.len > 0 ? float2{reciprocal(l[n][0]), reciprocal(l[n][1])} : float2{0.f, 0.f};
-                    // A copy of the loop for bf16 and one for codes take less time than a branch in it (8 x 2048 tokens 16.2 -> 15.5 us, 256 x 512 13.7 ->
-                    // 13.3), except where two blocks of e4m3 tokens a turn leave no registers for it (131071 tokens 34.4 -> 35.8)
+                    // A copy of the loop for bf16 and one for codes take less time than a branch in it (8 sequences of up to 4096 tokens 16.2 -> 15.5 us, 256 of
+                    // up to 512 13.7 -> 13.3), except where two blocks of e4m3 tokens a turn leave no registers for it (131071 tokens 34.4 -> 35.8)
                     constexpr int kAtOnce = kE4m3 && kM == 2 ? 1 : kD / 16;
 #pragma unroll
                     for (int c = 0; c < kD / 16; c += kAtOnce)
