@@ -36,13 +36,14 @@ struct CacheGrid {
     int lanes_log2;                   // lanes of a row
     int tokens;                       // tokens of a block's turn
     int64_t turns;                    // of all blocks
+    int step_tokens, step_rest;       // a step of a block's threads: whole tokens, rows beside them
+    int token_magic;                  // 2^16 / a token's rows, rounded up: row * token_magic / 2^16 is the token of any row below 256
     int blocks;
 };
 
 // Rows of a block, one behind the other: token, keys then values, head.  A thread goes through them in steps of as many as the block takes at a time.
 struct RowAt {
     int token, rest;
-    __device__ __forceinline__ RowAt(int row, int rows_of_token) : token(row / rows_of_token), rest(row - token * rows_of_token) {}
     __device__ __forceinline__ void step(int tokens, int more, int rows_of_token) {
         token += tokens;
         rest += more;
@@ -60,7 +61,11 @@ struct CacheLane {
     int64_t row_step;                 // a step of `steps.token` tokens, where heads stay
     __device__ __forceinline__ CacheLane(const CacheView& c, const CacheRows& x, const CacheGrid& grid)
         : tid(threadIdx.x), sub(tid & ((1 << grid.lanes_log2) - 1)), step(kCacheThreads >> grid.lanes_log2), heads(c.kv_heads), chunks(c.dim >> 3),
-          lanes(1 << grid.lanes_log2), at(tid >> grid.lanes_log2, 2 * c.kv_heads), steps(step, 2 * c.kv_heads) {}
+          lanes(1 << grid.lanes_log2), steps{grid.step_tokens, grid.step_rest} {
+        const int row = tid >> grid.lanes_log2;
+        at.token = row * grid.token_magic >> 16;
+        at.rest = row - at.token * 2 * heads;
+    }
     __device__ __forceinline__ void place(const CacheView& c, const CacheRows& x, int64_t token0) {
         const bool values = at.rest >= heads;
         const int head = values ? at.rest - heads : at.rest;
@@ -197,6 +202,7 @@ kv_cache_write_kernel(CacheView c, CacheRows x, const int* slots, CacheGrid grid
                 }
             }
         }
+        if (turn + gridDim.x >= grid.turns) break;
         put(slot, side ^ 1);
         __syncthreads();
     }
@@ -310,6 +316,7 @@ kv_cache_read_kernel(CacheView c, CacheRows y, const int* tables, int64_t ld_tab
                 }
             }
         }
+        if (turn + gridDim.x >= grid.turns) break;
         put(next, side ^ 1);
         __syncthreads();
     }
@@ -321,9 +328,13 @@ kv_cache_read_kernel(CacheView c, CacheRows y, const int* tables, int64_t ld_tab
 // a quarter beside them.  (Reading up to 1404 tokens of 10 heads of 80 for 11 sequences: 6 or 12 tokens 21.5 us, the power of two 28.2; 206 MB of 4
 // heads of 128: 32 tokens 38.8, 16 tokens 40.9; writing 16842 tokens of 2 heads of 128: 32 tokens 7.5, 64, too few for the chip's blocks, 11.2.)
 static CacheGrid cache_grid(const CacheView& c, int64_t rows, int deep) {
-    CacheGrid g = {1, 1, 0, 0};
+    CacheGrid g = {1, 1, 0, 0, 0, 0, 0};
     while ((16 << g.lanes_log2) < c.dim) ++g.lanes_log2;
-    const int at_once = std::min((kCacheThreads >> g.lanes_log2) * deep / (2 * c.kv_heads), kMaxTokens);
+    const int step = kCacheThreads >> g.lanes_log2, rows_of_token = 2 * c.kv_heads;
+    g.step_tokens = step / rows_of_token;
+    g.step_rest = step % rows_of_token;
+    g.token_magic = 65536 / rows_of_token + 1;
+    const int at_once = std::min(step * deep / rows_of_token, kMaxTokens);
     const int64_t sms = sm_count(), spread = (rows + sms - 1) / sms;
     if (spread <= at_once) {
         g.tokens = (int)spread;
