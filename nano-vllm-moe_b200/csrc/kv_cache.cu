@@ -35,10 +35,13 @@ constexpr int kMaxEnds = 1024;        // sequences whose ends fit a block's shar
 struct CacheGrid {
     int lanes_log2;                   // lanes of a row
     int tokens;                       // tokens of a block's turn
-    int64_t turns;                    // of all blocks
+    int turns;                        // of all blocks
     int step_tokens, step_rest;       // a step of a block's threads: whole tokens, rows beside them
     int token_magic;                  // 2^16 / a token's rows, rounded up: row * token_magic / 2^16 is the token of any row below 256
+    uint32_t page_magic;              // a token's page: token * page_magic / 2^(32 + page_shift) below 2^31; 0: pages of one token
+    int page_shift;
     int blocks;
+    __device__ __forceinline__ int page_of(int token) const { return page_magic ? (int)(__umulhi((uint32_t)token, page_magic) >> page_shift) : token; }
 };
 
 // Rows of a block, one behind the other: token, keys then values, head.  A thread goes through them in steps of as many as the block takes at a time.
@@ -66,7 +69,7 @@ struct CacheLane {
         at.token = row * grid.token_magic >> 16;
         at.rest = row - at.token * 2 * heads;
     }
-    __device__ __forceinline__ void place(const CacheView& c, const CacheRows& x, int64_t token0) {
+    __device__ __forceinline__ void place(const CacheView& c, const CacheRows& x, int token0) {
         const bool values = at.rest >= heads;
         const int head = values ? at.rest - heads : at.rest;
         cache = (values ? c.v : c.k) + head * c.sh;
@@ -74,7 +77,7 @@ struct CacheLane {
         row = (values ? x.v : x.k) + (token0 + at.token) * (values ? x.vt : x.kt) + head * (values ? x.vh : x.kh);
         row_step = steps.token * (values ? x.vt : x.kt);
     }
-    __device__ __forceinline__ void next(const CacheView& c, const CacheRows& x, int64_t token0) {
+    __device__ __forceinline__ void next(const CacheView& c, const CacheRows& x, int token0) {
         at.step(steps.token, steps.rest, 2 * heads);
         if (steps.rest == 0) row += row_step;
         else place(c, x, token0);
@@ -133,20 +136,20 @@ kv_cache_write_kernel(CacheView c, CacheRows x, const int* slots, CacheGrid grid
     const bool low = word0 < origin.chunks, high = word1 < origin.chunks, odd = origin.sub & 1;
     const int code = (origin.sub >> 1) + (odd ? origin.lanes >> 1 : 0);  // of 16 codes
     pdl_wait();
-    auto tokens_of = [&](int64_t turn) {
-        const int64_t left = x.rows - turn * grid.tokens;
-        return left < grid.tokens ? (int)left : grid.tokens;
+    auto tokens_of = [&](int turn) {
+        const int left = (int)x.rows - turn * grid.tokens;
+        return left < grid.tokens ? left : grid.tokens;
     };
-    auto slot_of = [&](int64_t turn) { return turn < grid.turns && origin.tid < tokens_of(turn) ? ld_dep(slots + turn * grid.tokens + origin.tid) : -1; };
+    auto slot_of = [&](int turn) { return turn < grid.turns && origin.tid < tokens_of(turn) ? ld_dep(slots + turn * grid.tokens + origin.tid) : -1; };
     auto put = [&](int slot, int side) {
         if (origin.tid >= kMaxTokens) return;
-        const int64_t page = slot / c.block_size;
+        const int page = grid.page_of(slot);
         s_at[side][origin.tid] = slot < 0 ? TokenAt{-1, -1} : token_at(c, page, slot - page * c.block_size, status);
     };
     int slot = slot_of(blockIdx.x), side = 0;
     bool placed = false;
-    for (int64_t turn = blockIdx.x; turn < grid.turns; turn += gridDim.x, side ^= 1) {
-        const int64_t token0 = turn * grid.tokens;
+    for (int turn = blockIdx.x; turn < grid.turns; turn += gridDim.x, side ^= 1) {
+        const int token0 = turn * grid.tokens;
         const int tokens = tokens_of(turn), rows = tokens * 2 * c.kv_heads;
         CacheLane me = origin;
         me.place(c, x, token0);
@@ -210,7 +213,7 @@ kv_cache_write_kernel(CacheView c, CacheRows x, const int* slots, CacheGrid grid
 
 // The sequence b with cu[b] <= row < cu[b + 1], or -1.
 template <class Ends>
-__device__ __forceinline__ int sequence_of(Ends cu, int batch, int64_t row) {
+__device__ __forceinline__ int sequence_of(Ends cu, int batch, int row) {
     int lo = 0, hi = batch;                        // cu[lo] <= row < cu[hi], if there is one
     if (row < cu(0) || row >= cu(batch)) return -1;
     while (hi - lo > 1) {
@@ -237,24 +240,25 @@ kv_cache_read_kernel(CacheView c, CacheRows y, const int* tables, int64_t ld_tab
         for (int i = tid; i <= batch; i += kCacheThreads) s_ends[i] = ld_dep(cu + i);
     __syncthreads();
     // A token's page and offset; the page on its way.
-    struct Looked { int64_t off; int page; bool there; };
-    auto look = [&](int64_t turn) {
+    struct Looked { int off, page; bool there; };
+    auto look = [&](int turn) {
         Looked l = {0, -1, false};
-        const int64_t row = turn * grid.tokens + tid;
-        if (turn >= grid.turns || tid >= grid.tokens || row >= y.rows) return l;
-        int b;
-        int64_t at;
+        const int row = turn * grid.tokens + tid;
+        if (turn >= grid.turns || tid >= grid.tokens || row >= (int)y.rows) return l;
+        int b, from = 0;
         if (batch <= kMaxEnds) {
             b = sequence_of([&](int i) { return s_ends[i]; }, batch, row);
-            at = b < 0 ? 0 : row - s_ends[b];
+            if (b >= 0) from = s_ends[b];
         } else {
             b = sequence_of([&](int i) { return ld_dep(cu + i); }, batch, row);
-            at = b < 0 ? 0 : row - ld_dep(cu + b);
+            if (b >= 0) from = ld_dep(cu + b);
         }
         if (b < 0) return l;
-        const int64_t i = (uint32_t)at / (uint32_t)c.block_size;              // (a division of 64 bits is a hundred instructions, every turn)
-        l.off = at - i * c.block_size;
         l.there = true;
+        const int at = (int)((uint32_t)row - (uint32_t)from);
+        if (at < 0) return l;                                            // (only where a sequence begins below 0: no page)
+        const int i = grid.page_of(at);
+        l.off = at - i * c.block_size;
         if (i < max_pages) l.page = ld_dep(tables + b * ld_tables + i);
         return l;
     };
@@ -264,8 +268,8 @@ kv_cache_read_kernel(CacheView c, CacheRows y, const int* tables, int64_t ld_tab
     int side = 0;
     put(look(blockIdx.x), side);
     __syncthreads();
-    for (int64_t turn = blockIdx.x; turn < grid.turns; turn += gridDim.x, side ^= 1) {
-        const int64_t token0 = turn * grid.tokens;
+    for (int turn = blockIdx.x; turn < grid.turns; turn += gridDim.x, side ^= 1) {
+        const int token0 = turn * grid.tokens;
         const int tokens = y.rows - token0 < grid.tokens ? (int)(y.rows - token0) : grid.tokens;
         const Looked next = look(turn + gridDim.x);
         CacheLane me = origin;
@@ -328,12 +332,19 @@ kv_cache_read_kernel(CacheView c, CacheRows y, const int* tables, int64_t ld_tab
 // a quarter beside them.  (Reading up to 1404 tokens of 10 heads of 80 for 11 sequences: 6 or 12 tokens 21.5 us, the power of two 28.2; 206 MB of 4
 // heads of 128: 32 tokens 38.8, 16 tokens 40.9; writing 16842 tokens of 2 heads of 128: 32 tokens 7.5, 64, too few for the chip's blocks, 11.2.)
 static CacheGrid cache_grid(const CacheView& c, int64_t rows, int deep) {
-    CacheGrid g = {1, 1, 0, 0, 0, 0, 0};
+    CacheGrid g = {};
+    g.lanes_log2 = g.tokens = 1;
     while ((16 << g.lanes_log2) < c.dim) ++g.lanes_log2;
     const int step = kCacheThreads >> g.lanes_log2, rows_of_token = 2 * c.kv_heads;
     g.step_tokens = step / rows_of_token;
     g.step_rest = step % rows_of_token;
     g.token_magic = 65536 / rows_of_token + 1;
+    if (c.block_size > 1) {                                              // 2^(31 + l) / block_size, rounded up, where 2^l is the power of two from block_size on
+        int l = 1;
+        while ((1ll << l) < c.block_size) ++l;
+        g.page_magic = (uint32_t)(((1ull << (31 + l)) + c.block_size - 1) / c.block_size);
+        g.page_shift = l - 1;
+    }
     const int at_once = std::min(step * deep / rows_of_token, kMaxTokens);
     const int64_t sms = sm_count(), spread = (rows + sms - 1) / sms;
     if (spread <= at_once) {
@@ -352,7 +363,7 @@ static CacheGrid cache_grid(const CacheView& c, int64_t rows, int deep) {
         consider(at_once, 1);
         if (rows >= 2 * at_once * sms * kHeld) consider(2 * at_once, 2);
     }
-    g.turns = (rows + g.tokens - 1) / g.tokens;
+    g.turns = (int)((rows + g.tokens - 1) / g.tokens);
     const int64_t most = kCacheBlocks * sms;
     g.blocks = (int)(g.turns < most ? g.turns : most);
     return g;
