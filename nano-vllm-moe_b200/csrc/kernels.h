@@ -278,6 +278,23 @@ cudaError_t launch_swap_w8a16(const SwapPlan& plan, const UmmaArgs& a, const voi
 
 // ---- paged key-value cache (kv_cache.cu, paged_attention.cu) ----
 // fp8lin_kv_cache as the kernels take it: checked, strides of the rows in bytes, those of dimensions of one element 0.
+// n / d for n from 0 to 2^31 - 1 by a multiplication: 2^(31 + l) / d, rounded up, where 2^l is the power of two from d on.
+struct Divisor {
+    uint32_t magic = 0;            // 0: d is 1
+    int shift = 0;
+    Divisor() = default;
+    explicit Divisor(int d) {
+        if (d <= 1) return;
+        int l = 1;
+        while ((1ll << l) < d) ++l;
+        magic = (uint32_t)(((1ull << (31 + l)) + d - 1) / d);
+        shift = l - 1;
+    }
+#ifdef __CUDACC__
+    __device__ __forceinline__ int quotient(int n) const { return magic ? (int)(__umulhi((uint32_t)n, magic) >> shift) : n; }
+#endif
+};
+
 struct CacheView {
     unsigned char* k;
     unsigned char* v;
@@ -313,6 +330,7 @@ struct AttnArgs {
     int* status;
     int* counters;
     float* partial;
+    Divisor by_page, by_segments, by_parts;      // block_size; a sequence's segments; parts of a group of query heads
 };
 size_t paged_attention_scratch(int64_t heads, int64_t kv_heads, int64_t dim, bool e4m3);
 cudaError_t launch_paged_attention(const AttnArgs& a, cudaStream_t stream);

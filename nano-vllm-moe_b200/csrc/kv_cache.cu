@@ -38,10 +38,8 @@ struct CacheGrid {
     int turns;                        // of all blocks
     int step_tokens, step_rest;       // a step of a block's threads: whole tokens, rows beside them
     int token_magic;                  // 2^16 / a token's rows, rounded up: row * token_magic / 2^16 is the token of any row below 256
-    uint32_t page_magic;              // a token's page: token * page_magic / 2^(32 + page_shift) below 2^31; 0: pages of one token
-    int page_shift;
     int blocks;
-    __device__ __forceinline__ int page_of(int token) const { return page_magic ? (int)(__umulhi((uint32_t)token, page_magic) >> page_shift) : token; }
+    Divisor by_page;                  // block_size
 };
 
 // Rows of a block, one behind the other: token, keys then values, head.  A thread goes through them in steps of as many as the block takes at a time.
@@ -143,7 +141,7 @@ kv_cache_write_kernel(CacheView c, CacheRows x, const int* slots, CacheGrid grid
     auto slot_of = [&](int turn) { return turn < grid.turns && origin.tid < tokens_of(turn) ? ld_dep(slots + turn * grid.tokens + origin.tid) : -1; };
     auto put = [&](int slot, int side) {
         if (origin.tid >= kMaxTokens) return;
-        const int page = grid.page_of(slot);
+        const int page = grid.by_page.quotient(slot);
         s_at[side][origin.tid] = slot < 0 ? TokenAt{-1, -1} : token_at(c, page, slot - page * c.block_size, status);
     };
     int slot = slot_of(blockIdx.x), side = 0;
@@ -257,7 +255,7 @@ kv_cache_read_kernel(CacheView c, CacheRows y, const int* tables, int64_t ld_tab
         l.there = true;
         const int at = (int)((uint32_t)row - (uint32_t)from);
         if (at < 0) return l;                                            // (only where a sequence begins below 0: no page)
-        const int i = grid.page_of(at);
+        const int i = grid.by_page.quotient(at);
         l.off = at - i * c.block_size;
         if (i < max_pages) l.page = ld_dep(tables + b * ld_tables + i);
         return l;
@@ -339,12 +337,7 @@ static CacheGrid cache_grid(const CacheView& c, int64_t rows, int deep) {
     g.step_tokens = step / rows_of_token;
     g.step_rest = step % rows_of_token;
     g.token_magic = 65536 / rows_of_token + 1;
-    if (c.block_size > 1) {                                              // 2^(31 + l) / block_size, rounded up, where 2^l is the power of two from block_size on
-        int l = 1;
-        while ((1ll << l) < c.block_size) ++l;
-        g.page_magic = (uint32_t)(((1ull << (31 + l)) + c.block_size - 1) / c.block_size);
-        g.page_shift = l - 1;
-    }
+    g.by_page = Divisor(c.block_size);
     const int at_once = std::min(step * deep / rows_of_token, kMaxTokens);
     const int64_t sms = sm_count(), spread = (rows + sms - 1) / sms;
     if (spread <= at_once) {
