@@ -172,6 +172,14 @@ at::Tensor empty(at::IntArrayRef shape, at::ScalarType dtype, c10::Device device
     return at::detail::empty_cuda(shape, dtype, device, c10::nullopt);
 }
 
+// `shape` of a tensor's memory, from element `from` on.
+at::Tensor part_of(const at::Tensor& whole, at::IntArrayRef shape, int64_t from) {
+    at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(whole.storage()), whole.key_set(), whole.dtype());
+    t.unsafeGetTensorImpl()->set_storage_offset(from);
+    t.unsafeGetTensorImpl()->set_sizes_contiguous(shape);
+    return t;
+}
+
 at::Tensor empty_like_rows(const at::Tensor& x, int64_t n, at::ScalarType dtype) {
     if (x.dim() == 2) {
         const int64_t shape[2] = {x.size(0), n};
@@ -583,8 +591,12 @@ PyObject* py_kv_cache_read(PyObject*, PyObject* const* a, Py_ssize_t na) {
         const at::Tensor* ko = optional_tensor(a[7], "k_out");
         const at::Tensor* vo = optional_tensor(a[8], "v_out");
         const c10::cuda::CUDAGuard device(on);
-        const at::Tensor k = ko ? *ko : empty({rows, c.num_kv_heads, c.head_dim}, at::kBFloat16, on);
-        const at::Tensor v = vo ? *vo : empty({rows, c.num_kv_heads, c.head_dim}, at::kBFloat16, on);
+        // One allocation for both: a second one takes a small call a sixth of its time.
+        const int64_t shape[3] = {rows, c.num_kv_heads, c.head_dim}, half = rows * c.num_kv_heads * c.head_dim;
+        at::Tensor both;
+        if (!ko || !vo) both = empty({(ko || vo) ? half : 2 * half}, at::kBFloat16, on);
+        const at::Tensor k = ko ? *ko : part_of(both, shape, 0);
+        const at::Tensor v = vo ? *vo : part_of(both, shape, ko ? 0 : half);
         check_heads(k, c.num_kv_heads, c.head_dim, on, "k_out");
         check_heads(v, c.num_kv_heads, c.head_dim, on, "v_out");
         if (k.size(0) != rows || v.size(0) != rows) throw ValueError("k_out and v_out must have the given number of rows");

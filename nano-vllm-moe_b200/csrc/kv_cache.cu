@@ -324,6 +324,12 @@ kv_cache_read_kernel(CacheView c, CacheRows y, const int* tables, int64_t ld_tab
     }
 }
 
+static int lanes_log2(int dim) {
+    int l = 1;
+    while ((16 << l) < dim) ++l;
+    return l;
+}
+
 // Tokens of a block's turn: an SM's share where that is less than what a block's threads take at once, `deep` rows each.  Else that many, or
 // the power of two below, or twice as many where all blocks that the chip holds still get a turn, whichever leaves the SM with the most turns
 // the least to do.  A turn costs, in terms of the bytes of what the threads take at once, those of its tokens, one for each step of its threads and
@@ -331,8 +337,8 @@ kv_cache_read_kernel(CacheView c, CacheRows y, const int* tables, int64_t ld_tab
 // heads of 128: 32 tokens 38.8, 16 tokens 40.9; writing 16842 tokens of 2 heads of 128: 32 tokens 7.5, 64, too few for the chip's blocks, 11.2.)
 static CacheGrid cache_grid(const CacheView& c, int64_t rows, int deep) {
     CacheGrid g = {};
-    g.lanes_log2 = g.tokens = 1;
-    while ((16 << g.lanes_log2) < c.dim) ++g.lanes_log2;
+    g.lanes_log2 = lanes_log2(c.dim);
+    g.tokens = 1;
     const int step = kCacheThreads >> g.lanes_log2, rows_of_token = 2 * c.kv_heads;
     g.step_tokens = step / rows_of_token;
     g.step_rest = step % rows_of_token;
@@ -364,7 +370,7 @@ static CacheGrid cache_grid(const CacheView& c, int64_t rows, int deep) {
 
 // Whether four rows a thread would leave some without any: the chip's threads hold the call's rows once.
 static bool few_rows(const CacheView& c, int64_t rows) {
-    return rows * 2 * c.kv_heads <= (int64_t)sm_count() * 4 * (kCacheThreads >> cache_grid(c, rows, 1).lanes_log2);
+    return rows * 2 * c.kv_heads <= (int64_t)sm_count() * 4 * (kCacheThreads >> lanes_log2(c.dim));
 }
 
 template <class Kernel, class... Args>

@@ -415,6 +415,28 @@ def test_reads_of_every_length(pkg, kv_heads, dim, e4m3):
             assert torch.equal(got, torch.cat([*want, torch.full_like(got[:3], 7.0)]))
 
 
+@pytest.mark.parametrize("rows", [0, 1, 37])
+def test_results_of_a_read_are_tensors_of_their_own(pkg, rows):
+    c = pkg.PagedKVCache(4, 16, 3, 48)
+    k, v = rows_of(64, 3, 48, seed=6)
+    c.write(k, v, torch.arange(64, dtype=torch.int32, device="cuda"))
+    tables, cu = torch.arange(4, dtype=torch.int32, device="cuda")[None], torch.tensor([0, rows], dtype=torch.int32, device="cuda")
+    mine = torch.empty(rows, 3, 48, dtype=torch.bfloat16, device="cuda")
+    with torch.inference_mode():
+        pairs = [c.read(tables, cu, rows), kernels().kv_cache_read(c.k, c.v, tables, cu, rows, v_out=mine), kernels().kv_cache_read(c.k, c.v, tables, cu, rows, k_out=mine)]
+    pairs[1:1] = [c.read(tables, cu, rows)]
+    for got in pairs[:2]:
+        assert torch.equal(got[0], k[:rows]) and torch.equal(got[1], v[:rows])
+        for x in got:
+            assert x.shape == (rows, 3, 48) and x.is_contiguous() and not x.requires_grad and x._base is None
+    assert torch.equal(pairs[2][0], k[:rows]) and torch.equal(pairs[3][1], v[:rows])
+    a, b = pairs[1]
+    a.zero_()                                             # (in place: one does not reach into the other)
+    assert torch.equal(b, v[:rows]) and torch.equal(b.clone().float(), v[:rows].float())
+    del a, pairs
+    assert torch.equal(b, v[:rows])
+
+
 @pytest.mark.parametrize("order", ["heads", "tokens", "wide"])
 @pytest.mark.parametrize("e4m3", [False, True])
 def test_read_of_a_batch(e4m3, order):
