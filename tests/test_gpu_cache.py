@@ -1,6 +1,7 @@
 """The paged cache and the decode attention on the GPU against their definitions in 64 bits."""
 import importlib
 import math
+import threading
 
 import numpy as np
 import pytest
@@ -570,6 +571,70 @@ def test_calls_on_several_streams():
     torch.cuda.synchronize()
     for w, g in zip(want, got):
         assert all(torch.equal(w, x) for x in g)
+
+
+def test_calls_of_several_threads():
+    Kn = kernels()
+    caches = [Cache([9000 + 555 * i, 40, 7], 4, 64, 32, bool(i % 2), seed=i) for i in range(3)]
+    q = queries(3, 16, 64)
+    want = [check(c, q) for c in caches]
+    wrong = []
+
+    def work(c, w):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(20):
+                    if not torch.equal(Kn.paged_attention(q, *c.args(), **c.scales()), w):
+                        wrong.append("differs")
+        except Exception as e:                            # noqa: BLE001  (shown by the assertion below)
+            wrong.append(repr(e))
+
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=work, args=x) for x in zip(caches, want)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+def test_tables_and_lengths_of_any_layout(e4m3):
+    """Slices of wider tables, tables of one page per sequence, of none."""
+    Kn = kernels()
+    c = Cache([40, 0, 700, 16], 2, 64, 16, e4m3, seed=8)
+    q = queries(4, 14, 64)
+    want = check(c, q)
+    wide = torch.full((4, c.tables.shape[1] + 13), -9, dtype=torch.int32, device="cuda")
+    wide[:, 5:5 + c.tables.shape[1]] = c.tables
+    lens = torch.stack([c.lens, c.lens + 1])[0]
+    assert torch.equal(Kn.paged_attention(q, c.k, c.v, wide[:, 5:5 + c.tables.shape[1]], lens, **c.scales()), want)
+    c = Cache([16, 3, 0, 9], 2, 64, 16, e4m3, seed=9)
+    want = check(c, q)
+    assert torch.equal(Kn.paged_attention(q, c.k, c.v, c.tables[:, :1], c.lens, **c.scales()), want)
+    assert torch.equal(Kn.paged_attention(q, c.k, c.v, c.tables[:, 0].contiguous()[:, None], c.lens, **c.scales()), want)
+    assert not Kn.paged_attention(q, c.k, c.v, c.tables[:, :0], torch.zeros_like(c.lens), **c.scales()).any()
+
+
+def test_a_cache_of_all_layers(pkg):
+    """The layout in which an engine allocates it: [2, layers, blocks, tokens, heads, channels] in one tensor."""
+    Kn, layers, (blocks, block, heads, dim) = kernels(), 3, (9, 16, 2, 64)
+    whole = torch.zeros(2, layers, blocks, block, heads, dim, dtype=torch.bfloat16, device="cuda")
+    tables = torch.tensor([[3, 0, 8], [5, 2, 7]], dtype=torch.int32, device="cuda")
+    lens = [40, 17]
+    rows = [tuple(rows_of(57, heads, dim, seed=i)) for i in range(layers)]
+    slots = torch.cat([tables[b].long().repeat_interleave(block)[:n] * block + torch.arange(n, device="cuda") % block for b, n in enumerate(lens)]).to(torch.int32)
+    for (k, v), kc, vc in zip(rows, whole[0], whole[1]):
+        Kn.kv_cache_write(k, v, slots, kc, vc)
+    cu = torch.tensor([0, 40, 57], dtype=torch.int32, device="cuda")
+    own = pkg.PagedKVCache(blocks, block, heads, dim)
+    q = queries(2, 14, dim)
+    for (k, v), kc, vc in zip(rows, whole[0], whole[1]):
+        got = Kn.kv_cache_read(kc, vc, tables, cu, 57)
+        assert torch.equal(got[0], k) and torch.equal(got[1], v)
+        own.write(k, v, slots)
+        n = torch.tensor(lens, dtype=torch.int32, device="cuda")
+        assert torch.equal(Kn.paged_attention(q, kc, vc, tables, n), Kn.paged_attention(q, own.k, own.v, tables, n))
 
 
 @pytest.mark.parametrize("e4m3", [False, True])
