@@ -13,12 +13,12 @@
 // holds 16, even lanes in the row's first half and odd ones in its second, and neighbours exchange half of theirs on the way.
 // (Reading 206 MB back took 46 us with a lane's 16 channels side by side on both sides, which writes half sectors, and 50 with two
 // times eight codes a lane.)
-// A thread has kDeep rows in flight: four, or one where the call has no more for it (2.3 instead of 3.4 us for 64 tokens of 4 heads).
+// A thread has kDeep rows in flight: four, or one where the call has hardly more for it (few_rows).
 // A block takes a few tokens at a time with all their heads, keys and values; what a token needs (its slot; its sequence, page and
 // offset) is looked up once, a turn early: looked up when it was needed, it took longer than the rows.
 //
-// Measured (B200, in a row of calls, inputs larger than L2): writing 51 MB (16384 tokens of 4 heads of 128, to codes) 14.9 us, 17 MB
-// 3.8; reading 206 MB of codes back 39 us, 5.3 TB/s, 134 MB of bf16 24 us, 5.5 TB/s.  A kernel that only copies 34 MB takes 8.5 us.
+// Measured (B200, in a row of calls, inputs larger than L2): writing 51 MB (16384 tokens of 4 heads of 128, to codes) 14.4 us, 17 MB
+// of bf16 3.45, 64 tokens 2.1; reading 206 MB of codes back 37 us, 5.5 TB/s, 134 MB of bf16 24 us, 5.6 TB/s, 777 tokens 2.95.  A kernel that only copies 34 MB takes 8.5 us.
 #include <algorithm>
 
 #include "common.cuh"
@@ -368,9 +368,11 @@ static CacheGrid cache_grid(const CacheView& c, int64_t rows, int deep) {
     return g;
 }
 
-// Whether four rows a thread would leave some without any: the chip's threads hold the call's rows once.
+// Whether a row a thread is the better way: up to a third more rows than the threads of six blocks per SM hold at once (1031 tokens of 16 heads
+// of 128 written in 3.45 us, four rows a thread 3.9; 17 sequences of 276 to 552 tokens of 2 heads of 128 read in 4.4, 5.3; with twice as many
+// rows as this it is the other way round: 36 of up to 438 tokens of 4 heads 6.2 with four rows, 7.3 with one).
 static bool few_rows(const CacheView& c, int64_t rows) {
-    return rows * 2 * c.kv_heads <= (int64_t)sm_count() * 4 * (kCacheThreads >> lanes_log2(c.dim));
+    return rows * 2 * c.kv_heads <= (int64_t)sm_count() * 8 * (kCacheThreads >> lanes_log2(c.dim));
 }
 
 template <class Kernel, class... Args>
