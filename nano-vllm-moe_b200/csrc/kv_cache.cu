@@ -13,11 +13,12 @@
 // holds 16, even lanes in the row's first half and odd ones in its second, and neighbours exchange half of theirs on the way.
 // (Reading 206 MB back took 46 us with a lane's 16 channels side by side on both sides, which writes half sectors, and 50 with two
 // times eight codes a lane.)
-// A thread has kDeep rows in flight: four, or one where the call has hardly more for it (few_rows).
+// A thread has kDeep rows in flight: two of a write, whose rows are two words a lane (16384 tokens of 4 heads 13.1 us, with four 14.4; 5000 tokens
+// 4.8, 6.4), four of a read (206 MB 37 us, with two 44, with three 39), or one where the call has hardly more for it (few_rows).
 // A block takes a few tokens at a time with all their heads, keys and values; what a token needs (its slot; its sequence, page and
 // offset) is looked up once, a turn early: looked up when it was needed, it took longer than the rows.
 //
-// Measured (B200, in a row of calls, inputs larger than L2): writing 51 MB (16384 tokens of 4 heads of 128, to codes) 14.4 us, 17 MB
+// Measured (B200, in a row of calls, inputs larger than L2): writing 51 MB (16384 tokens of 4 heads of 128, to codes) 13.1 us, 17 MB
 // of bf16 3.45, 64 tokens 2.1; reading 206 MB of codes back 37 us, 5.5 TB/s, 134 MB of bf16 24 us, 5.6 TB/s, 777 tokens 2.95.  A kernel that only copies 34 MB takes 8.5 us.
 #include <algorithm>
 
@@ -28,8 +29,9 @@ namespace fp8lin {
 
 constexpr int kCacheThreads = 256;
 constexpr int kMaxTokens = 64;        // tokens of a block's turn
-constexpr int kCacheBlocks = 8;       // blocks of a launch per SM, twice what it holds
-constexpr int kHeld = 4;              // blocks that an SM holds at a time, of threads with four rows in flight
+constexpr int kCacheBlocks = 8;       // blocks of a launch per SM
+// Blocks that an SM holds at a time, by the rows that their threads have in flight.
+constexpr int held(int deep) { return deep == 1 ? 6 : deep == 2 ? 5 : 4; }
 constexpr int kMaxEnds = 1024;        // sequences whose ends fit a block's shared memory
 
 struct CacheGrid {
@@ -125,7 +127,7 @@ __device__ __forceinline__ TokenAt token_at(const CacheView& c, int64_t page, in
 }
 
 template <bool kE4m3, int kDeep>
-__global__ void __launch_bounds__(kCacheThreads, kDeep == 1 ? 6 : 4)
+__global__ void __launch_bounds__(kCacheThreads, held(kDeep))
 kv_cache_write_kernel(CacheView c, CacheRows x, const int* slots, CacheGrid grid, int* status) {
     __shared__ TokenAt s_at[2][kMaxTokens];
     pdl_launch_dependents();
@@ -223,7 +225,7 @@ __device__ __forceinline__ int sequence_of(Ends cu, int batch, int row) {
 }
 
 template <bool kE4m3, int kDeep>
-__global__ void __launch_bounds__(kCacheThreads, kDeep == 1 ? 6 : 4)
+__global__ void __launch_bounds__(kCacheThreads, held(kDeep))
 kv_cache_read_kernel(CacheView c, CacheRows y, const int* tables, int64_t ld_tables, int64_t max_pages, const int* cu, int batch, CacheGrid grid, int* status) {
     __shared__ TokenAt s_at[2][kMaxTokens];
     __shared__ int s_ends[kMaxEnds + 1];
@@ -334,7 +336,8 @@ static int lanes_log2(int dim) {
 // the power of two below, or twice as many where all blocks that the chip holds still get a turn, whichever leaves the SM with the most turns
 // the least to do.  A turn costs, in terms of the bytes of what the threads take at once, those of its tokens, one for each step of its threads and
 // a quarter beside them.  (Reading up to 1404 tokens of 10 heads of 80 for 11 sequences: 6 or 12 tokens 21.5 us, the power of two 28.2; 206 MB of 4
-// heads of 128: 32 tokens 38.8, 16 tokens 40.9; writing 16842 tokens of 2 heads of 128: 32 tokens 7.5, 64, too few for the chip's blocks, 11.2.)
+// heads of 128: 32 tokens 38.8, 16 tokens 40.9; writing 16842 tokens of 2 heads of 128, four rows in
+// flight: 32 tokens 7.5, 64, too few for the chip's blocks, 11.2.)
 static CacheGrid cache_grid(const CacheView& c, int64_t rows, int deep) {
     CacheGrid g = {};
     g.lanes_log2 = lanes_log2(c.dim);
@@ -360,7 +363,7 @@ static CacheGrid cache_grid(const CacheView& c, int64_t rows, int deep) {
         while (2 * power <= at_once) power *= 2;
         consider(power, 1);
         consider(at_once, 1);
-        if (rows >= 2 * at_once * sms * kHeld) consider(2 * at_once, 2);
+        if (rows >= 2 * at_once * sms * held(deep)) consider(2 * at_once, 2);
     }
     g.turns = (int)((rows + g.tokens - 1) / g.tokens);
     const int64_t most = kCacheBlocks * sms;
@@ -369,7 +372,7 @@ static CacheGrid cache_grid(const CacheView& c, int64_t rows, int deep) {
 }
 
 // Whether a row a thread is the better way: up to a third more rows than the threads of six blocks per SM hold at once (1031 tokens of 16 heads
-// of 128 written in 3.45 us, four rows a thread 3.9; 17 sequences of 276 to 552 tokens of 2 heads of 128 read in 4.4, 5.3; with twice as many
+// of 128 written in 3.45 us, with four rows a thread 3.9; 17 sequences of 276 to 552 tokens of 2 heads of 128 read in 4.4, 5.3; with twice as many
 // rows as this it is the other way round: 36 of up to 438 tokens of 4 heads 6.2 with four rows, 7.3 with one).
 static bool few_rows(const CacheView& c, int64_t rows) {
     return rows * 2 * c.kv_heads <= (int64_t)sm_count() * 8 * (kCacheThreads >> lanes_log2(c.dim));
@@ -389,9 +392,9 @@ static cudaError_t launch_cache(Kernel kernel, int blocks, cudaStream_t stream, 
 
 cudaError_t launch_kv_cache_write(const CacheView& c, const CacheRows& x, const int* slots, int* status, cudaStream_t stream) {
     const bool few = few_rows(c, x.rows);
-    const CacheGrid g = cache_grid(c, x.rows, few ? 1 : 4);
-    auto kernel = c.e4m3 ? (few ? kv_cache_write_kernel<true, 1> : kv_cache_write_kernel<true, 4>)
-                         : (few ? kv_cache_write_kernel<false, 1> : kv_cache_write_kernel<false, 4>);
+    const CacheGrid g = cache_grid(c, x.rows, few ? 1 : 2);
+    auto kernel = c.e4m3 ? (few ? kv_cache_write_kernel<true, 1> : kv_cache_write_kernel<true, 2>)
+                         : (few ? kv_cache_write_kernel<false, 1> : kv_cache_write_kernel<false, 2>);
     return launch_cache(kernel, g.blocks, stream, c, x, slots, g, status);
 }
 
