@@ -386,9 +386,10 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
     // Nothing that the loop needs is waited for in it: a load queues behind all the copies that the SM's warps have asked for, some
     // 2.5 us.  So lengths and queries are asked for a segment early, and pages come 32 table entries at a time, a lane each, also
     // early: those from page_base on, the 32 behind them, a sequence's first for its next head, and the next sequence's.
+    // (The walk runs ahead of what there is, behind the last tile of the batch into a sequence that does not exist: `entry` tells it.)
     int pages = 0, pages_behind = 0, pages_first = 0, page_base = 0, page_at = 0, page_off = 0;
     int next_len = 0, next_pages = 0, after_len = 0;                // of the sequences behind in.b, behind at.b
-    auto entry = [&](int b, int64_t i) { return i < a.max_pages ? ld_dep(a.tables + (int64_t)b * a.ld_tables + i) : -1; };
+    auto entry = [&](int b, int64_t i) { return b < a.batch && i < a.max_pages ? ld_dep(a.tables + (int64_t)b * a.ld_tables + i) : -1; };
     auto look_at = [&](int b) {
         if (b < a.batch) {
             next_len = ld_dep(a.lens + b);
