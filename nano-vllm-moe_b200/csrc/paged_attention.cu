@@ -23,7 +23,11 @@
 // P is split into two numbers of 16 bits, so the weights are good to 2^-16 (bf16) or 2^-21 (f16) instead of 2^-8, for a third
 // of the matrix instructions and 1% of the time.
 // e4m3 codes are widened to f16 (exact) behind ldmatrix.  Queries are scaled by a power of two into f16's range; a token's
-// key scale multiplies its scores, its value scale its weight, relative to a power of two near the largest so far.
+// key scale multiplies its scores, its value scale its weight.  That product is what has to fit f16: per query head it is relative to
+// a power of two near the largest product so far, wherever the largest score and the largest scale are, so a token's part of the
+// result is off by 2^-21 of itself or 2^-31 of the largest part.  (Weights below 2^-126 of the largest are none;
+// scales below 2^kLeast lose digits.  Relative to the largest scale alone it took 256 sequences of up to 512 tokens 13.35 us instead of
+// 13.55, a group of 12 heads 31.0 instead of 32.0, the long and the full batches the same, and lost what a quiet token gave beside a louder value.)
 //
 // Measured (B200, in a row of calls, inputs larger than L2): 311 MB of an e4m3 cache (64 sequences of 1000 to 8192 tokens, 28 heads on 4 of 128) 62 us,
 // 5.0 TB/s; 282 MB of a bf16 one (32 sequences of 100 to 2048, 16 heads on 16) 56 us, 5.0 TB/s; 138 MB (one sequence of 131071, e4m3) 35 us,
@@ -113,6 +117,17 @@ constexpr float kNone = -3.402823466e38f;
 // Weights are relative to a score that is at most 2^kSlack below the largest: it follows the maximum only where that
 // runs away from it, so that the sums are rescaled once or twice per segment and not with every new maximum.
 constexpr float kSlack = 8.f;
+// e4m3: the same for weights times value scales, in f16: 2^kTop for the largest that a reference was made of, 2^(kTop + kSlack) at most.
+constexpr float kTop = 6.f;
+// Smaller value scales (the formula's are 2^-36 at least) count as this one where references are made.
+constexpr float kLeast = -100.f;
+__device__ __forceinline__ float log2_approx(float x) {
+    float r;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ float power_of_2(int e) { return __int_as_float((e + 127) << 23); }                     // e from -126 to 127
+__device__ __forceinline__ int exponent(float x) { return (int)(__float_as_uint(x) >> 23) - 127; }                 // of a positive number
 __device__ __forceinline__ float warp_max(float x) {
     float r;
     asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(x));
@@ -516,8 +531,9 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
     const Result result(a);
     uint32_t q[kD / 16][kN][2];
     float o[kD / 16][kN][4], m[kN][2], l[kN][2], to_score[kN][2];
-    float v_most = 0.f, v_up = 0.f;                                                // ... the largest scale that goes with it, and what they are multiplied by
-    int value_exp = 15;                                                            // exponent field that the values' scales are relative to
+    // e4m3: sums are those of weights times value scales times v_up, a power of two.  As long as scores are at most `gap` above m and scales at
+    // most v_most, no product is more than 2^kSlack times its reference, whichever score goes with whichever scale.
+    float v_up[kN][2], gap = kSlack, v_most = 0.f;
     // Queries are asked for one segment early where registers allow: they queue behind the tiles that the SM's warps have asked for.
     constexpr bool kQueriesEarly = kN == 1 && kD <= 128;
     uint32_t q_next[kQueriesEarly ? kD / 16 : 1][kN][2];
@@ -544,9 +560,8 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
         }
     };
     auto begin_segment = [&](bool first) {
-        value_exp = 15;
         v_most = 0.f;
-        v_up = __uint_as_float(245u << 23);
+        gap = kSlack;
         if constexpr (kQueriesEarly) {
             if (first) load_queries(q_next, at);
 #pragma unroll
@@ -585,7 +600,11 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
                 to_score[n][0] = to_score[n][1] = base;
             }
 #pragma unroll
-            for (int i = 0; i < 2; ++i) { m[n][i] = kNone; l[n][i] = 0.f; }
+            for (int i = 0; i < 2; ++i) {
+                m[n][i] = kNone;
+                l[n][i] = 0.f;
+                v_up[n][i] = power_of_2((int)(kTop - kLeast));
+            }
 #pragma unroll
             for (int c = 0; c < kD / 16; ++c)
 #pragma unroll
@@ -598,7 +617,9 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
     const uint32_t k_lane = k_r * kRow + swizzle(k_r, mi >> 1) * 16, v_lane = v_r * kRow + swizzle(v_r, kE4m3 ? mi >> 1 : mi & 1) * 16;
     auto words_on = [](uint32_t lane_at, int w) { return (lane_at ^ ((w & 7) * 16)) + (w & ~7) * 16; };
     constexpr int kLoads = kD / (kE4m3 ? 32 : 16);                                 // of a block's keys (or values)
-    constexpr bool kEarly = kM * kLoads <= 8;                                      // values to registers in front of the softmax
+    // Values to registers in front of the softmax, where there are registers for them (with 16 warps per CTA they spill: 256 sequences of
+    // up to 512 tokens 13.7 us, without 13.55)
+    constexpr bool kEarly = kM * kLoads <= 8 && kWarps <= 8;
     auto work_on = [&](int stage) {
         const uint32_t ks = my_ring_at + stage * S::kStageBytes, k_at = ks + k_lane, v_at = ks + kTile * kRow + v_lane;
         auto load_keys = [&](uint32_t (&f)[4], int h, int x) { ldmatrix4(f, words_on(k_at, 2 * x) + h * kBlock * kRow); };
@@ -680,7 +701,7 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
                 top[n][i] = fmaxf(s[0][n][i], s[0][n][2 + i]);
 #pragma unroll
                 for (int h = 1; h < kM; ++h) top[n][i] = fmaxf(top[n][i], fmaxf(s[h][n][i], s[h][n][2 + i]));
-                raised |= top[n][i] > m[n][i] + kSlack;
+                raised |= top[n][i] > (kE4m3 ? __fadd_rd(m[n][i], gap) : m[n][i] + kSlack);
             }
         float v_top = 0.f;
         if (kE4m3) {
@@ -689,26 +710,42 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
             raised |= v_top > v_most;
         }
         if (__any_sync(0xffffffffu, raised)) {
-            float down = 1.f;
-            if (kE4m3) {                                                           // the next power of two above the largest scale
-                const int e = __reduce_max_sync(0xffffffffu, max(value_exp, (int)(__float_as_uint(v_top) >> 23)));
-                down = exp2_approx((float)(value_exp - e));
-                value_exp = e;
-                v_most = __uint_as_float((uint32_t)e << 23 | 0x7fffffu);
-                v_up = __uint_as_float((uint32_t)(260 - e) << 23);                 // 2^(6 - (e - 127)): weights times scales below 2^15
+            float v_log[kM][2], most = 0.f;                                        // (v_most: the tile's, so that a louder one is forgotten when it has passed)
+            if (kE4m3) {
+                const uint32_t e = __reduce_max_sync(0xffffffffu, __float_as_uint(v_top) >> 23);
+                v_most = __uint_as_float(e << 23 | 0x7fffffu);
+                most = (float)((int)e - 126);
+                gap = kSlack;
+#pragma unroll
+                for (int h = 0; h < kM; ++h)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) v_log[h][i] = fmaxf(log2_approx(fabsf(v_scale[h][i])), kLeast);
             }
+            auto lanes_max = [](float x) {
+                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+                return fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+            };
 #pragma unroll
             for (int n = 0; n < kN; ++n)
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    float x = top[n][i];
-                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
-                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
-                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-                    x = fmaxf(m[n][i], x);
-                    const float f = exp2_approx(m[n][i] - x), fd = f * down;
+                    const float x = fmaxf(m[n][i], lanes_max(top[n][i])), down = m[n][i] - x, f = exp2_approx(down);
+                    float fd = f;
                     m[n][i] = x;
                     l[n][i] *= f;
+                    if (kE4m3) {
+                        float y = -INFINITY;                                       // of the scores' distances from m: scores may be far larger than the scales' logarithms
+#pragma unroll
+                        for (int h = 0; h < kM; ++h)
+#pragma unroll
+                            for (int r = 0; r < 2; ++r) y = fmaxf(y, s[h][n][2 * r + i] - x + v_log[h][r]);
+                        const float before = kTop - (float)exponent(v_up[n][i]) + down;
+                        const float ref = fminf(fmaxf(ceilf(fmaxf(before, lanes_max(y))), kLeast), 129.f);     // (beyond them: infinities and NaN)
+                        fd = exp2_approx(before - ref);
+                        v_up[n][i] = power_of_2((int)(kTop - ref));
+                        gap = fminf(gap, ref + kSlack - most);
+                    }
 #pragma unroll
                     for (int c = 0; c < kD / 16; ++c) { o[c][n][i] *= fd; o[c][n][2 + i] *= fd; }
                 }
@@ -716,8 +753,6 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
         uint32_t hi[kM][kN][2], lo[kM][kN][2];
 #pragma unroll
         for (int h = 0; h < kM; ++h) {
-            float up[2] = {1.f, 1.f};
-            if (kE4m3) { up[0] = v_scale[h][0] * v_up; up[1] = v_scale[h][1] * v_up; }
 #pragma unroll
             for (int n = 0; n < kN; ++n)
 #pragma unroll
@@ -727,8 +762,9 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
                     for (int i = 0; i < 2; ++i) {
                         p[i] = exp2_approx(s[h][n][2 * r + i] - m[n][i]);
                         l[n][i] += p[i];
-                        if (kE4m3) p[i] *= up[r];
                     }
+                    if (kE4m3)                                                     // (v_up first: it undoes what a scale far from 1 does)
+                        unpack_f32x2(mul_f32x2(mul_f32x2(pack_f32x2(p[0], p[1]), pack_f32x2(v_up[n][0], v_up[n][1])), pack_f32x2(v_scale[h][r], v_scale[h][r])), p[0], p[1]);
                     split2<kE4m3>(p[0], p[1], hi[h][n][r], lo[h][n][r]);
                     hi[h][n][r] = transposed(hi[h][n][r]);
                     lo[h][n][r] = transposed(lo[h][n][r]);
@@ -800,7 +836,6 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
         from = from + 1 == kStages ? 0 : from + 1;
         const bool ends = at.t + 1 == at.tiles, last = at.place + 1 + (ends ? kBegin : 0) >= span;
         if (ends || last) {
-            const float back = kE4m3 ? __uint_as_float((uint32_t)(value_exp - 6) << 23) : 1.f;
 #pragma unroll
             for (int n = 0; n < kN; ++n)
 #pragma unroll
@@ -808,9 +843,11 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
                     l[n][j] += __shfl_xor_sync(0xffffffffu, l[n][j], 4);
                     l[n][j] += __shfl_xor_sync(0xffffffffu, l[n][j], 8);
                     l[n][j] += __shfl_xor_sync(0xffffffffu, l[n][j], 16);
-                    if (kE4m3)
+                    if (kE4m3) {
+                        const float back = power_of_2(-exponent(v_up[n][j]));
 #pragma unroll
                         for (int c = 0; c < kD / 16; ++c) { o[c][n][j] *= back; o[c][n][2 + j] *= back; }
+                    }
                 }
             if (ends && from_start) {                                               // the whole segment was this warp's
 #pragma unroll
