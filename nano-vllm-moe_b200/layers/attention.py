@@ -60,9 +60,11 @@ class PagedAttention(DirectModule):
         self.cache: PagedKVCache | None = None
 
     def _attend(self, q, k, v, slot_mapping, block_tables, context_lens, out_scale):
+        cache = self.cache
+        if cache is not None and cache.k.size(2) != self.num_kv_heads:
+            raise ValueError(f"the cache holds {cache.k.size(2)} key heads, the layer has num_kv_heads={self.num_kv_heads}")
         if not q.is_cuda:
             raise RuntimeError("fp8lin PagedAttention requires CUDA")
-        cache = self.cache
         if cache is None:
             raise RuntimeError("PagedAttention has no cache: assign a PagedKVCache to its .cache first")
         host, rows, d = _lib.host(), q.shape[0], self.head_dim
