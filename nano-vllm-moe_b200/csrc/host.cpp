@@ -586,7 +586,9 @@ PyObject* py_kv_cache_read(PyObject*, PyObject* const* a, Py_ssize_t na) {
         const int32_t* cp = int32_of(cu, 1, on, "cu_seqlens");
         const int64_t rows = PyLong_AsLongLong(a[4]);
         if (PyErr_Occurred()) return nullptr;
-        if (rows < 0) throw ValueError("rows must not be negative");
+        // (what the library would refuse, in front of the memory for it)
+        if (rows < 0 || rows > (1ll << 30)) throw ValueError("rows must be from 0 to 2^30");
+        if (c.num_kv_heads > 65535 || c.head_dim > 256) throw ValueError("bad cache shape: at most 65535 key heads of at most 256 channels");
         if (cu.size(0) != tables.size(0) + 1) throw ValueError("cu_seqlens must have one value more than block_tables has rows");
         const at::Tensor* ko = optional_tensor(a[7], "k_out");
         const at::Tensor* vo = optional_tensor(a[8], "v_out");
