@@ -202,6 +202,8 @@ class RowParallelLinear(LinearBase):
     #    one barrier, every rank sums locally.  (tp - 1) times the payload per rank: only sensible between two ranks
     #    (down at M = 16384: 697 us).
     # False = always the NCCL all-reduce, as the reference.
+    # The peer forms are for bfloat16 activations of W8A8 layers.  W8A16 layers, and codes (a QuantizedActivation, as the attention of
+    # a decode step hands them on) of any number of rows, take the all-reduce whatever is set here: the same sums.
     # defer_gather (reduce-scatter form only): forward returns once the GEMM (with its scatter) is enqueued; the
     # barrier, the sum and the all-gather run on a side stream, so that the caller's next kernels -- work that does not
     # read this output, e.g. the next micro-batch's or an independent linear's GEMM -- run while NVLink carries the
@@ -401,7 +403,7 @@ class RowParallelLinear(LinearBase):
         if self.tp_size == 1:
             return self.apply_linear(x, bias)
         reduce = self.tp_size > 1 and bool(self.reduce_results)
-        if not isinstance(x, torch.Tensor):             # codes of a decode step: a few rows, summed by the all-reduce
+        if not isinstance(x, torch.Tensor):             # codes: summed by the all-reduce (see peer_reduce)
             if self.reduce_results == "scatter":
                 raise ValueError("reduce_results='scatter' takes bfloat16 activations, not codes")
             y = self.apply_linear(x, bias)
