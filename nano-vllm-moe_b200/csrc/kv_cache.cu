@@ -13,8 +13,9 @@
 // holds 16, even lanes in the row's first half and odd ones in its second, and neighbours exchange half of theirs on the way.
 // (Reading 206 MB back took 46 us with a lane's 16 channels side by side on both sides, which writes half sectors, and 50 with two
 // times eight codes a lane.)
-// A thread has kDeep rows in flight: two of a write, whose rows are two words a lane (16384 tokens of 4 heads 13.1 us, with four 14.4; 5000 tokens
-// 4.8, 6.4), four of a read (206 MB 37 us, with two 44, with three 39), or one where the call has hardly more for it (few_rows).
+// A thread has kDeep rows in flight: two of a write, whose rows are two words a lane (to codes: 16384 tokens of 4 heads of 128 13.1 us, with four 14.4; 5000
+// tokens 4.8, 6.4; in bf16 it is the other way round where heads leave threads without a row: 6000 tokens of 10 heads of 80 9.1, with four 8.8), four
+// of a read (206 MB 37 us, with two 44, with three 39), or one where the call has hardly more for it (few_rows).
 // A block takes a few tokens at a time with all their heads, keys and values; what a token needs (its slot; its sequence, page and
 // offset) is looked up once, a turn early: looked up when it was needed, it took longer than the rows.
 //
@@ -335,9 +336,9 @@ static int lanes_log2(int dim) {
 // Tokens of a block's turn: an SM's share where that is less than what a block's threads take at once, `deep` rows each.  Else that many, or
 // the power of two below, or twice as many where all blocks that the chip holds still get a turn, whichever leaves the SM with the most turns
 // the least to do.  A turn costs, in terms of the bytes of what the threads take at once, those of its tokens, one for each step of its threads and
-// a quarter beside them.  (Reading up to 1404 tokens of 10 heads of 80 for 11 sequences: 6 or 12 tokens 21.5 us, the power of two 28.2; 206 MB of 4
-// heads of 128: 32 tokens 38.8, 16 tokens 40.9; writing 16842 tokens of 2 heads of 128, four rows in
-// flight: 32 tokens 7.5, 64, too few for the chip's blocks, 11.2.)
+// a quarter beside them.  (Reading up to 1404 tokens of 10 heads of 80 for 11 sequences: 6 or 12 tokens 15.6 us, the power of two 18.1; 206 MB of 4
+// heads of 128: 32 tokens 37.0, 16 tokens 38.2; writing 5000 tokens of 4 heads of 128 to codes: 8 tokens 4.8, 16, too few for the chip's blocks, 6.6;
+// 50000 tokens: 16 tokens 32.9, 8 tokens 37.0.)
 static CacheGrid cache_grid(const CacheView& c, int64_t rows, int deep) {
     CacheGrid g = {};
     g.lanes_log2 = lanes_log2(c.dim);
@@ -371,11 +372,18 @@ static CacheGrid cache_grid(const CacheView& c, int64_t rows, int deep) {
     return g;
 }
 
-// Whether a row a thread is the better way: up to a third more rows than the threads of six blocks per SM hold at once (1031 tokens of 16 heads
-// of 128 written in 3.45 us, with four rows a thread 3.9; 17 sequences of 276 to 552 tokens of 2 heads of 128 read in 4.4, 5.3; with twice as many
-// rows as this it is the other way round: 36 of up to 438 tokens of 4 heads 6.2 with four rows, 7.3 with one).
-static bool few_rows(const CacheView& c, int64_t rows) {
-    return rows * 2 * c.kv_heads <= (int64_t)sm_count() * 8 * (kCacheThreads >> lanes_log2(c.dim));
+// Whether a row a thread is the better way: while blocks of as many tokens as their threads take at once, a row each, are at most `most_even` per SM where
+// the heads divide those rows, `most_odd` where some threads have none (10 heads of 80: 20 of 32 rows; of codes, not where a token alone is
+// more than that).  Measured:
+// writes, 7 and 2: 937 tokens of 16 heads of 128 to codes 4.5 us with one row, 4.65 with two, 1184 tokens 5.0 and 4.3 (bf16 3.8 and 3.5); 150
+// tokens of 10 heads of 80 in bf16 1.9 and 2.1, 600 tokens 3.0 and 2.6, 1500 tokens 5.15 and 3.3; 394 tokens of 24 heads of 96 to codes 4.9 and 5.4;
+// reads, 8 and 2 (codes 5): 17 sequences of 276 to 552 tokens of 2 heads of 128 4.3 with one row, 5.3 with four, 36 of up to 438 tokens of 4 heads 7.7
+// and 6.1; 150 tokens of 10 heads of 80 in bf16 2.4 and 2.8, 600 tokens 3.6 and 3.3 (from codes 4.3 and 4.5), 1136 tokens from codes 5.9 and 5.7.
+static bool few_rows(const CacheView& c, int64_t tokens, int most_even, int most_odd) {
+    const int step = kCacheThreads >> lanes_log2(c.dim), rows_of_token = 2 * c.kv_heads;
+    const bool even = step % rows_of_token == 0 || rows_of_token % step == 0 || (c.e4m3 && rows_of_token > step);
+    const int64_t blocks = rows_of_token <= step ? (tokens + step / rows_of_token - 1) / (step / rows_of_token) : tokens * ((rows_of_token + step - 1) / step);
+    return blocks <= (int64_t)sm_count() * (even ? most_even : most_odd);
 }
 
 template <class Kernel, class... Args>
@@ -391,7 +399,7 @@ static cudaError_t launch_cache(Kernel kernel, int blocks, cudaStream_t stream, 
 }
 
 cudaError_t launch_kv_cache_write(const CacheView& c, const CacheRows& x, const int* slots, int* status, cudaStream_t stream) {
-    const bool few = few_rows(c, x.rows);
+    const bool few = few_rows(c, x.rows, 7, 2);
     const CacheGrid g = cache_grid(c, x.rows, few ? 1 : 2);
     auto kernel = c.e4m3 ? (few ? kv_cache_write_kernel<true, 1> : kv_cache_write_kernel<true, 2>)
                          : (few ? kv_cache_write_kernel<false, 1> : kv_cache_write_kernel<false, 2>);
@@ -400,7 +408,7 @@ cudaError_t launch_kv_cache_write(const CacheView& c, const CacheRows& x, const 
 
 cudaError_t launch_kv_cache_read(const CacheView& c, const CacheRows& y, const int* tables, int64_t ld_tables, int64_t max_pages, const int* cu_seqlens,
                                  int64_t batch, int* status, cudaStream_t stream) {
-    const bool few = few_rows(c, y.rows);
+    const bool few = few_rows(c, y.rows, 8, c.e4m3 ? 5 : 2);
     const CacheGrid g = cache_grid(c, y.rows, few ? 1 : 4);
     auto kernel = c.e4m3 ? (few ? kv_cache_read_kernel<true, 1> : kv_cache_read_kernel<true, 4>)
                          : (few ? kv_cache_read_kernel<false, 1> : kv_cache_read_kernel<false, 4>);
