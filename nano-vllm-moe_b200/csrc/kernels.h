@@ -278,7 +278,8 @@ cudaError_t launch_swap_w8a16(const SwapPlan& plan, const UmmaArgs& a, const voi
 
 // ---- paged key-value cache (kv_cache.cu, paged_attention.cu) ----
 // fp8lin_kv_cache as the kernels take it: checked, strides of the rows in bytes, those of dimensions of one element 0.
-// n / d for n from 0 to 2^31 - 1 by a multiplication: 2^(31 + l) / d, rounded up, where 2^l is the power of two from d on.
+// n / d for n from 0 to 2^31 - 1 by a multiplication: 2^(31 + l) / d, rounded up, where 2^l is the power of two from d on (Granlund and
+// Montgomery, "Division by invariant integers using multiplication", 1994).
 struct Divisor {
     uint32_t magic = 0;            // 0: d is 1
     int shift = 0;

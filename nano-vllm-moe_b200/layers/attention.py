@@ -42,7 +42,8 @@ class PagedKVCache:
         _lib.host().kv_cache_write(k, v, slot_mapping, self.k, self.v, self.k_scale, self.v_scale)
 
     def read(self, block_tables: torch.Tensor, cu_seqlens: torch.Tensor, rows: int) -> tuple[torch.Tensor, torch.Tensor]:
-        """bfloat16 (k, v) [rows, kv_heads, head_dim]: the first tokens of the sequences, one sequence behind the other."""
+        """bfloat16 (k, v) [rows, kv_heads, head_dim]: the first tokens of the sequences, one sequence behind the other.  Both lie in one
+        new piece of memory: either keeps all of it alive, and is saved with all of it (``clone`` what is to be kept alone)."""
         return _lib.host().kv_cache_read(self.k, self.v, block_tables, cu_seqlens, rows, self.k_scale, self.v_scale, None, None)
 
 

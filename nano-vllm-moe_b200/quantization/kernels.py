@@ -312,7 +312,7 @@ def kv_cache_read(k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: to
     """The cached tokens of a batch of sequences as bfloat16 (k, v) [rows, kv_heads, head_dim], one sequence behind the other:
     sequence b gets the rows from ``cu_seqlens[b]`` to ``cu_seqlens[b + 1]`` (int32, on the device), and its first tokens.
     Rows behind the last sequence (``rows`` may be more, as in a captured graph) are left as they were.  Without ``k_out`` and
-    ``v_out`` both are parts of one new piece of memory.  ``block_tables``: int32
+    ``v_out`` both are parts of one new piece of memory, which either keeps alive.  ``rows``: at most 2^30.  ``block_tables``: int32
     [batch, pages]; entries behind a sequence's last page may hold anything."""
     return _lib.host().kv_cache_read(k_cache, v_cache, block_tables, cu_seqlens, rows, k_scale, v_scale, k_out, v_out)
 
