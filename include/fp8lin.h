@@ -350,8 +350,9 @@ int fp8lin_kv_cache_read(const fp8lin_kv_cache* cache, const int32_t* block_tabl
  * the split of a long sequence (and with it the last bits) depends on the lengths of the whole batch.  An infinity or NaN among
  * a sequence's own keys and values makes what it reaches non-finite, as do values whose sum of up to 256 times
  * their size leaves fp32's range; nothing behind a context's end is read.  Weights are good to 2^-16 (bf16 caches) or 2^-21 (e4m3) of
- * themselves; of an e4m3 cache a token's part of the result is also off by up to 2^-31 of the largest product of a
- * weight and its row's largest value, weights below 2^-126 of the largest are none, and value scales below 2^-100 lose digits.
+ * themselves, and those below 2^-126 of the largest are none; of an e4m3 cache a token's part of the result is also off by up to
+ * 2^-31 of the largest product of a weight and 448 of its row's value scale (by the formula the row's largest value, 1e-8 where that is
+ * smaller), and value scales below 2^-100 lose digits.
  * out may be q itself (bf16, the same rows: ld_out = q_stride_row, q_stride_head = head_dim); apart from that it shares no memory
  * with what the call reads.  context_lens and block_tables stay as they are until the call has run.
  * workspace: fp8lin_paged_attention_workspace_bytes, zero-filled once, rules as for the linears. */

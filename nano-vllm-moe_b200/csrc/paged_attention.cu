@@ -26,7 +26,7 @@
 // e4m3 codes are widened to f16 (exact) behind ldmatrix.  Queries are scaled by a power of two into f16's range; a token's
 // key scale multiplies its scores, its value scale its weight.  That product is what has to fit f16: per query head it is relative to
 // a power of two near the largest product so far, wherever the largest score and the largest scale are, so a token's part of the
-// result is off by 2^-21 of itself or 2^-31 of the largest product of a weight and its row's largest value.  (Weights below 2^-126 of the largest are none;
+// result is off by 2^-21 of itself or 2^-31 of the largest product of a weight and 448 of its row's value scale.  (Weights below 2^-126 of the largest are none;
 // scales below 2^kLeast lose digits.  Relative to the largest scale alone it took 256 sequences of up to 512 tokens 13.35 us instead of
 // 13.55, a group of 12 heads 31.0 instead of 32.0, the long and the full batches the same, and lost what a quiet token gave beside a louder value.)
 //
