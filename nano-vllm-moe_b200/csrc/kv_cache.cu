@@ -372,18 +372,18 @@ static CacheGrid cache_grid(const CacheView& c, int64_t rows, int deep) {
     return g;
 }
 
-// Whether a row a thread is the better way: while blocks of as many tokens as their threads take at once, a row each, are at most `most_even` per SM where
-// the heads divide those rows, `most_odd` where some threads have none (10 heads of 80: 20 of 32 rows; of codes, not where a token alone is
-// more than that).  Measured:
-// writes, 7 and 2: 937 tokens of 16 heads of 128 to codes 4.5 us with one row, 4.65 with two, 1184 tokens 5.0 and 4.3 (bf16 3.8 and 3.5); 150
-// tokens of 10 heads of 80 in bf16 1.9 and 2.1, 600 tokens 3.0 and 2.6, 1500 tokens 5.15 and 3.3; 394 tokens of 24 heads of 96 to codes 4.9 and 5.4;
-// reads, 8 and 2 (codes 5): 17 sequences of 276 to 552 tokens of 2 heads of 128 4.3 with one row, 5.3 with four, 36 of up to 438 tokens of 4 heads 7.7
-// and 6.1; 150 tokens of 10 heads of 80 in bf16 2.4 and 2.8, 600 tokens 3.6 and 3.3 (from codes 4.3 and 4.5), 1136 tokens from codes 5.9 and 5.7.
-static bool few_rows(const CacheView& c, int64_t tokens, int most_even, int most_odd) {
-    const int step = kCacheThreads >> lanes_log2(c.dim), rows_of_token = 2 * c.kv_heads;
-    const bool even = step % rows_of_token == 0 || rows_of_token % step == 0 || (c.e4m3 && rows_of_token > step);
-    const int64_t blocks = rows_of_token <= step ? (tokens + step / rows_of_token - 1) / (step / rows_of_token) : tokens * ((rows_of_token + step - 1) / step);
-    return blocks <= (int64_t)sm_count() * (even ? most_even : most_odd);
+// Whether a row a thread is the better way: while blocks of as many tokens as their threads take at once, a row each, are at most `most` per SM; in bf16,
+// where a row costs little beside a block's start, at most 3 if more than a tenth of the threads has no row (10 heads of 80: 12 of 32).  Measured, one row
+// against several:
+// writes, 7: 937 tokens of 16 heads of 128 to codes 4.5 us and 4.65, 1184 tokens 5.0 and 4.3; 4000 of 3 heads 4.3 and 5.5, 6000 5.8 and 5.7; bf16
+// 4000 of 3 heads 3.3 and 3.4, 6000 4.3 and 3.6, 150 of 10 heads of 80 1.9 and 2.1, 600 3.0 and 2.6, 1500 5.15 and 3.3;
+// reads, 8: 17 sequences of 276 to 552 tokens of 2 heads of 128 from codes 4.3 and 5.3, 36 of up to 438 tokens of 4 heads 7.7 and 6.1; 900 tokens of 10 heads of
+// 80 5.3 and 5.7, 1700 7.75 and 6.2; bf16 4000 of 3 heads of 128 3.8 and 4.3, 6000 5.1 and 4.9, 150 of 10 heads of 80 2.4 and 2.8, 740 3.6 and 3.2.
+static bool few_rows(const CacheView& c, int64_t tokens, int most) {
+    const int step = kCacheThreads >> lanes_log2(c.dim), rows_of_token = 2 * c.kv_heads, at_once = step / rows_of_token;
+    const int64_t blocks = at_once ? (tokens + at_once - 1) / at_once : (tokens * rows_of_token + step - 1) / step;
+    const int used = at_once ? at_once * rows_of_token : rows_of_token, of = at_once ? step : (rows_of_token + step - 1) / step * step;
+    return blocks <= (int64_t)sm_count() * (c.e4m3 || used * 10ll >= of * 9ll ? most : 3);
 }
 
 template <class Kernel, class... Args>
@@ -399,7 +399,7 @@ static cudaError_t launch_cache(Kernel kernel, int blocks, cudaStream_t stream, 
 }
 
 cudaError_t launch_kv_cache_write(const CacheView& c, const CacheRows& x, const int* slots, int* status, cudaStream_t stream) {
-    const bool few = few_rows(c, x.rows, 7, 2);
+    const bool few = few_rows(c, x.rows, 7);
     const CacheGrid g = cache_grid(c, x.rows, few ? 1 : 2);
     auto kernel = c.e4m3 ? (few ? kv_cache_write_kernel<true, 1> : kv_cache_write_kernel<true, 2>)
                          : (few ? kv_cache_write_kernel<false, 1> : kv_cache_write_kernel<false, 2>);
@@ -408,7 +408,7 @@ cudaError_t launch_kv_cache_write(const CacheView& c, const CacheRows& x, const 
 
 cudaError_t launch_kv_cache_read(const CacheView& c, const CacheRows& y, const int* tables, int64_t ld_tables, int64_t max_pages, const int* cu_seqlens,
                                  int64_t batch, int* status, cudaStream_t stream) {
-    const bool few = few_rows(c, y.rows, 8, c.e4m3 ? 5 : 2);
+    const bool few = few_rows(c, y.rows, 8);
     const CacheGrid g = cache_grid(c, y.rows, few ? 1 : 4);
     auto kernel = c.e4m3 ? (few ? kv_cache_read_kernel<true, 1> : kv_cache_read_kernel<true, 4>)
                          : (few ? kv_cache_read_kernel<false, 1> : kv_cache_read_kernel<false, 4>);

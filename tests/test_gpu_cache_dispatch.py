@@ -9,8 +9,9 @@ pytestmark = pytest.mark.gpu
 
 
 @pytest.mark.parametrize("e4m3", [False, True])
-@pytest.mark.parametrize("kv_heads, dim, tokens", [(16, 128, (1036, 1037, 1184, 1185)), (4, 128, (4144, 4145, 4736, 4737)), (10, 80, (296, 297, 740, 741, 1500)),
-                                                   (24, 96, (148, 149, 518, 519, 592, 593)), (12, 64, (592, 593, 1480, 1481)), (64, 256, (64, 65, 74, 75, 150))])
+@pytest.mark.parametrize("kv_heads, dim, tokens", [(16, 128, (1036, 1037, 1184, 1185)), (4, 128, (4144, 4145, 4736, 4737)), (10, 80, (444, 445, 1036, 1037, 1184, 1185)),
+                                                   (24, 96, (296, 297, 690, 691, 789, 790)), (12, 64, (888, 889, 2072, 2073, 2368, 2369)), (3, 128, (5180, 5181, 5920, 5921)),
+                                                   (64, 256, (64, 65, 74, 75, 150))])
 def test_both_sides_of_a_limit(pkg, kv_heads, dim, tokens, e4m3):
     block, most = 16, max(tokens)
     for n in tokens:
