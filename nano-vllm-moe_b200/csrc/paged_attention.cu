@@ -711,7 +711,9 @@ paged_attention_kernel(AttnArgs a, int group, int parts) {
             raised |= v_top > v_most;
         }
         if (__any_sync(0xffffffffu, raised)) {
-            float v_log[kM][2], most = 0.f;                                        // (v_most: the tile's, so that a louder one is forgotten when it has passed)
+            // (v_most: the tile's, so that a louder one is forgotten when it has passed.  131071 tokens whose value scales vary by a factor of 3 at one standard
+            // deviation take 35.0 us, by 16 36.2.)
+            float v_log[kM][2], most = 0.f;
             if (kE4m3) {
                 const uint32_t e = __reduce_max_sync(0xffffffffu, __float_as_uint(v_top) >> 23);
                 v_most = __uint_as_float(e << 23 | 0x7fffffu);
